@@ -300,7 +300,7 @@ def _scale_plain(amax, code):
     else:
         part, exponent = torch.frexp(amax)                      # amax = part * 2^exponent, part in [0.5, 1)
         scale = torch.exp2((exponent - 9 + (part > 0.875)).double()).float()
-    return torch.where(amax.double() < TINY * (1 if code == "int8" else 256), 0.0, torch.where(scale < TINY, 0.0, scale))
+    return torch.where(scale < TINY, 0.0, scale)
 
 
 def _inverse_plain(scale):
