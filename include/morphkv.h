@@ -68,6 +68,35 @@ typedef struct mkv_pool {
     void *v_base[MKV_MAX_SEGMENTS]; /* device */
 } mkv_pool;
 
+/* Element types of the entry points that say so (the others go by elem_bytes: 2 = fp16, 4 = fp32). */
+typedef enum mkv_dtype { MKV_F16 = 0, MKV_BF16 = 1, MKV_F32 = 2 } mkv_dtype;
+
+/*
+ * A paged pool that holds its values in 8 bits, with one fp32 scale for each (block, layer, kv head), K and V apart.
+ * Codes: per segment [blocks, num_layers, num_kv_heads, block_size, head_dim], one byte each; scales: per segment
+ * [blocks, num_layers, num_kv_heads].  Segments and block ids as in mkv_pool.  A code q stands for q * scale.
+ *   MKV_Q8_INT8: scale = amax / 127, both in fp32; q = round-half-even(x * (1 / scale)).
+ *   MKV_Q8_E4M3: scale = the smallest power of two with amax <= 448 * scale; q = e4m3(x / scale).
+ * amax is taken over the block's tokens and the head's elements.  Scales below the smallest normal fp32 number are 0
+ * (and so are the codes); a block with a value that is not finite has the scale NaN.  No counterpart in the reference,
+ * whose pool is fp16 (worker/model.py:180-190).
+ */
+typedef enum mkv_q8_code { MKV_Q8_INT8 = 1, MKV_Q8_E4M3 = 2 } mkv_q8_code;
+typedef struct mkv_pool_q8 {
+    int32_t num_segments; /* 1 + number of elastic chunks, <= MKV_MAX_SEGMENTS */
+    int32_t code;         /* mkv_q8_code */
+    int32_t num_layers;
+    int32_t num_kv_heads;
+    int32_t block_size;
+    int32_t head_dim;
+    int64_t num_blocks_org;
+    int64_t chunk_blocks; /* ignored when num_segments == 1 */
+    void *k_base[MKV_MAX_SEGMENTS];  /* device */
+    void *v_base[MKV_MAX_SEGMENTS];  /* device */
+    float *k_scale[MKV_MAX_SEGMENTS]; /* device */
+    float *v_scale[MKV_MAX_SEGMENTS]; /* device */
+} mkv_pool_q8;
+
 /* ---- library --------------------------------------------------------- */
 int mkv_version(void);
 const char *mkv_status_string(int status);
@@ -315,6 +344,71 @@ int mkv_store_kv_prefill(int device, void *stream, const void *k, const void *v,
                          const mkv_pool *pool, const int32_t *block_table, int64_t table_stride,
                          const int32_t *seq_ids, const int32_t *start_locs, const int32_t *seq_lens,
                          int num_seqs, int max_seq_len, int cur_layer);
+
+/* ---- 8-bit pool -------------------------------------------------------- */
+/*
+ * The 8-bit counterparts of mkv_store_kv_decode / mkv_store_kv_prefill (the reference has fp16 pools only).
+ * k, v: device rows [tokens, num_kv_heads, head_dim] of `dtype`, elements and heads contiguous, consecutive tokens
+ * k_stride / v_stride elements apart.  table_stride = columns of the block table, num_rows = its rows.
+ * Prefill: every block a prompt touches gets its scale from the prompt's tokens alone; slots behind the prompt's end keep
+ * their bytes.  Prompt i takes rows [start_locs[i], start_locs[i] + seq_lens[i]) of k and v; rows at or behind
+ * num_tokens are not read.  max_seq_len only sizes the launch.
+ * Decode: token len-1 of every sequence is appended.  In the first slot of a block its scale starts from the new token;
+ * later the larger of the block's and the token's scale holds, and if that is the token's, the codes of the slots
+ * before it are rounded again to the new scale (int8: q * fl32(old * fl32(1 / new)); e4m3: q * old / new).
+ * A sequence given more than once: its last entry counts.  Sequences whose length is not positive, ids outside the
+ * table, positions behind the table's last column and blocks outside the pool are skipped.
+ */
+int mkv_store_kv_q8_prefill(int device, void *stream, const void *k, const void *v, int64_t k_stride, int64_t v_stride,
+                            int dtype, int64_t num_tokens, const mkv_pool_q8 *pool, const int32_t *block_table,
+                            int64_t table_stride, int num_rows, const int32_t *seq_ids, const int32_t *start_locs,
+                            const int32_t *seq_lens, int num_seqs, int max_seq_len, int cur_layer);
+int mkv_store_kv_q8_decode(int device, void *stream, const void *k, const void *v, int64_t k_stride, int64_t v_stride,
+                           int dtype, const mkv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
+                           int num_rows, const int32_t *seq_ids, const int32_t *seq_lens, int batch, int cur_layer);
+
+/*
+ * Cached tokens back into contiguous rows: token t in [begins[i], ends[i]) of sequence seq_ids[i] becomes row
+ * start_locs[i] + t - begins[i] of k and v ([num_out_rows, num_kv_heads, head_dim] of `dtype`, rounded once from
+ * q * scale).  Rows at or behind num_out_rows, and tokens whose page is not there (as above), are not written.
+ * max_len (the longest range) only sizes the launch.
+ */
+int mkv_load_kv_q8(int device, void *stream, void *k, void *v, int64_t k_stride, int64_t v_stride, int dtype,
+                   int64_t num_out_rows, const mkv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
+                   int num_rows, const int32_t *seq_ids, const int32_t *begins, const int32_t *ends,
+                   const int32_t *start_locs, int num_seqs, int max_len, int cur_layer);
+
+/*
+ * Decode attention over the 8-bit pool: one query token for each sequence, o = softmax(scale * q (s K)^T) (s V) in
+ * fp32, rounded once to `dtype`.  q: [batch, num_q_heads, head_dim], sequences q_stride elements apart; o contiguous.
+ * The call plans, attends and merges in ONE launch.  `workspace` (device, 256-byte aligned, at least
+ * mkv_attn_q8_workspace_bytes(...) bytes, whose first mkv_attn_q8_zero_bytes(...) bytes are zero before its first use and are
+ * left zero by every call, the error word excepted) must not be shared by calls that may overlap on the GPU.
+ * max_seq_len is an upper bound of the lengths that sizes the launch; longer sequences are still attended in full.
+ * Rows of sequences whose length is not positive are left as they were; tokens whose page is not there (as above) take
+ * no part, and bit 0 of the workspace's first word is set; a row left without any token is NaN.
+ * Fast path: fp16 or bf16, head_dim 64 or 128, block_size 16, 32, 64 ...; everything else (fp32 queries, head_dim <=
+ * 512, any block size) takes a plain kernel, which needs no workspace.
+ */
+size_t mkv_attn_q8_workspace_bytes(int device, int batch, int num_q_heads, int num_kv_heads, int head_dim);
+size_t mkv_attn_q8_zero_bytes(int device);
+int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_stride, void *o, int dtype,
+                           const mkv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride, int num_rows,
+                           const int32_t *seq_ids, const int32_t *seq_lens, int batch, int num_q_heads, int cur_layer,
+                           float softmax_scale, int max_seq_len, void *workspace, size_t workspace_bytes);
+
+/*
+ * Rotary embedding by position: pair j of every head of token t turns by the angle positions[t] * inv_freq[j]
+ * (64 bits, reduced to a fraction of a turn before it is rounded) and is scaled by attention_scale; computed in fp32,
+ * rounded once.  num_pairs = elements of inv_freq = rotary dimensions / 2; elements behind 2 * num_pairs pass through.
+ * Pairs are (j, j + num_pairs), or with interleaved != 0 (2j, 2j + 1).  strides (host, 8): elements between tokens and
+ * between heads of q, k, q_out, k_out.  q_out / k_out: q / k themselves (in place) or memory that overlaps neither.
+ * positions: int32 or int64 by positions_bytes.  The table-free counterpart of mkv_rotary_embedding.
+ */
+int mkv_rotary_positions(int device, void *stream, const void *q, const void *k, void *q_out, void *k_out,
+                         const int64_t *strides, const void *positions, int positions_bytes, const double *inv_freq,
+                         int num_pairs, int interleaved, float attention_scale, int64_t num_tokens, int num_q_heads,
+                         int num_kv_heads, int head_dim, int dtype);
 
 /* ---- block table ------------------------------------------------------ */
 /*

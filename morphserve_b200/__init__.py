@@ -12,6 +12,11 @@ Drop-in replacements, behind the reference's own Python names, for
               acquire_new_kvcache, ...}                   -> swiftllm_c
   elastic expand / release / compaction bookkeeping       -> server.memory_utils
 
+and, beside them, the same step over a cache held in 8 bits:
+
+  store_kvcache_q8, load_kvcache_q8, paged_attention_q8   -> worker.kernels.kv_q8
+  rotary_embedding_positions, rotary_inv_freq             -> worker.kernels.rotary_pos
+
 Everything runs in hand-written CUDA (``libmorphkv.so``, C ABI in
 ``include/morphkv.h``).  There is no Triton, no CPU path and no fallback:
 importing the package without the built library raises.
@@ -28,10 +33,12 @@ from .worker import block_manager, infer_state, kv_model
 from .worker.block_manager import BlockManager
 from .worker.infer_state import LlamaInferState
 from .worker.kv_model import KVCacheModelState
-from .worker.kernels import block_mgmt, kvcache_mgmt, paged_attn, rotary_emb
+from .worker.kernels import block_mgmt, kv_q8, kvcache_mgmt, paged_attn, rotary_emb, rotary_pos
+from .worker.kernels.kv_q8 import alloc_kvcache_q8, load_kvcache_q8, paged_attention_q8, store_kvcache_q8
 from .worker.kernels.kvcache_mgmt import set_fused_decode_append, store_kvcache
 from .worker.kernels.paged_attn import paged_attention, paged_attention_push, wait_ready
 from .worker.kernels.rotary_emb import rotary_embedding_inplace, set_fused_decode_rope, set_rope_rounding
+from .worker.kernels.rotary_pos import rotary_embedding_positions, rotary_inv_freq
 
 __version__ = "0.1.0"
 
@@ -81,5 +88,6 @@ def install_as_swiftllm(overwrite: bool = True) -> None:
 
 __all__ = ["paged_attention", "paged_attention_push", "wait_ready", "store_kvcache", "set_fused_decode_append",
            "rotary_embedding_inplace", "set_fused_decode_rope", "set_rope_rounding", "BlockManager", "LlamaInferState",
-           "KVCacheModelState",
+           "KVCacheModelState", "alloc_kvcache_q8", "store_kvcache_q8", "load_kvcache_q8", "paged_attention_q8",
+           "rotary_embedding_positions", "rotary_inv_freq",
            "swiftllm_c", "memory_utils", "install_as_swiftllm"]

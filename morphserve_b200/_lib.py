@@ -37,8 +37,26 @@ class MkvPool(C.Structure):
     ]
 
 
+class MkvPoolQ8(C.Structure):
+    _fields_ = [
+        ("num_segments", C.c_int32),
+        ("code", C.c_int32),
+        ("num_layers", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("block_size", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("num_blocks_org", C.c_int64),
+        ("chunk_blocks", C.c_int64),
+        ("k_base", C.c_void_p * MKV_MAX_SEGMENTS),
+        ("v_base", C.c_void_p * MKV_MAX_SEGMENTS),
+        ("k_scale", C.c_void_p * MKV_MAX_SEGMENTS),
+        ("v_scale", C.c_void_p * MKV_MAX_SEGMENTS),
+    ]
+
+
 _vp, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _pool = C.POINTER(MkvPool)
+_pool_q8 = C.POINTER(MkvPoolQ8)
 
 # name -> (restype, argtypes); must list every function of include/morphkv.h
 SIGNATURES = {
@@ -66,6 +84,16 @@ SIGNATURES = {
                                                    _i, _i, _i, _f, _i, _vp, _sz]),
     "mkv_store_kv_decode": (_i, [_i, _vp, _vp, _vp, _pool, _vp, _i64, _vp, _vp, _i, _i]),
     "mkv_store_kv_prefill": (_i, [_i, _vp, _vp, _vp, _pool, _vp, _i64, _vp, _vp, _vp, _i, _i, _i]),
+    "mkv_store_kv_q8_prefill": (_i, [_i, _vp, _vp, _vp, _i64, _i64, _i, _i64, _pool_q8, _vp, _i64, _i, _vp, _vp, _vp, _i, _i,
+                                     _i]),
+    "mkv_store_kv_q8_decode": (_i, [_i, _vp, _vp, _vp, _i64, _i64, _i, _pool_q8, _vp, _i64, _i, _vp, _vp, _i, _i]),
+    "mkv_load_kv_q8": (_i, [_i, _vp, _vp, _vp, _i64, _i64, _i, _i64, _pool_q8, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _i]),
+    "mkv_attn_q8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "mkv_attn_q8_zero_bytes": (_sz, [_i]),
+    "mkv_paged_attention_q8": (_i, [_i, _vp, _vp, _i64, _vp, _i, _pool_q8, _vp, _i64, _i, _vp, _vp, _i, _i, _i, _f, _i, _vp,
+                                    _sz]),
+    "mkv_rotary_positions": (_i, [_i, _vp, _vp, _vp, _vp, _vp, C.POINTER(_i64), _vp, _i, _vp, _i, _i, _f, _i64, _i, _i, _i,
+                                  _i]),
     "mkv_block_need": (_i, [_i, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
     "mkv_slab_upload": (_i, [_i, _vp, _sz, _vp, _sz]),
     "mkv_block_allocate": (_i, [_i, _vp, _vp, _i, _vp, _i64, _vp, _vp, _i, _i, _vp, _i64, _vp, _vp, _i64, _vp]),

@@ -112,10 +112,48 @@ def attn_workspace(dev: int, batch: int, hq: int, hkv: int, d: int, max_blocks: 
     return ws
 
 
+# Scratch of the 8-bit pool's attention (partial rows, arrival counters).  Outside a capture: one buffer per (device,
+# stream), as above, whose counters are zeroed once and left zero by every launch.  Inside a capture: a buffer of the
+# call's own, from the graph's memory, zeroed by a node of the graph - replays of two graphs may overlap, and a launch
+# outside them may run beside both.
+_workspaces_q8: dict = {}
+_q8_bytes_cache: dict = {}
+
+
+def workspace_q8(dev: int, stream: int, batch: int, hq: int, hkv: int, d: int):
+    """(tensor, bytes) for one launch on `stream`, which is the current stream of `dev`."""
+    key = (dev, batch, hq, hkv, d)
+    need = _q8_bytes_cache.get(key)
+    if need is None:
+        need = (int(lib.mkv_attn_q8_workspace_bytes(dev, batch, hq, hkv, d)), int(lib.mkv_attn_q8_zero_bytes(dev)))
+        if need[0] == 0:
+            raise RuntimeError("mkv_attn_q8_workspace_bytes failed")
+        _q8_bytes_cache[key] = need
+    nbytes, zero = need
+    if dev == torch.cuda.current_device():
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(dev):
+            capturing = torch.cuda.is_current_stream_capturing()
+    ws = None if capturing else _workspaces_q8.get((dev, stream))
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+        ws[:zero].zero_()
+        if not capturing:
+            if len(_workspaces_q8) >= _MAX_WORKSPACES and (dev, stream) not in _workspaces_q8:
+                _workspaces_q8.pop(next(iter(_workspaces_q8)))
+            _workspaces_q8[(dev, stream)] = ws
+    return ws, ws.numel()
+
+
 def read_attn_error_flags(dev: int) -> int:
     """Debug helper: the error words of every attention workspace of the device, OR-ed.  Bit 0 = a block-table
-    entry pointed outside the pool."""
+    entry pointed outside the pool.  (The 8-bit pool's launches inside captured graphs have words of their own, which
+    are not among them.)"""
     out = 0
+    for (d, _), ws in list(_workspaces_q8.items()):
+        if d == dev:
+            out |= int(ws[:4].view(torch.int32).item())
     for (d, _), ws in list(_workspaces.items()):
         if d != dev or ws.tensor is None:
             continue

@@ -1,0 +1,120 @@
+"""Rotary embedding by position, without tables: both pair layouts, part of the head, frequencies scaled for long
+contexts.
+
+``rotary_embedding_inplace`` (worker/kernels/rotary_emb.py:43-58) takes gathered fp16 cos/sin rows, rotates whole heads
+in the half layout and knows linear scaling only (worker/model.py:229-241).  Here the kernel forms the angles itself, in
+64 bits, from the tokens' positions and one frequency for each pair.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from ..._lib import check, lib
+from ._common import device_and_stream, require_cuda
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}       # mkv_dtype
+
+
+def rotary_inv_freq(model_config, device="cuda"):
+    """``(inv_freq, attention_scale)`` of a model: radians a position for each pair (float64 on ``device``) and the
+    factor on sines and cosines.
+
+    Read from ``model_config``: ``head_dim``, ``rope_theta`` (default 10000), ``partial_rotary_factor`` (default 1: the
+    part of the head that is rotated), ``max_position_embeddings`` and ``rope_scaling``: nothing, a number (linear, as in
+    worker/model.py:232-238), or a mapping with ``rope_type`` (or ``type``) and ``factor``:
+
+      default          no scaling
+      linear           positions divided by ``factor``
+      ntk              base * factor^(d / (d - 2))
+      llama3           by bands of turns over ``original_max_position_embeddings``: above ``high_freq_factor`` kept, below
+                       ``low_freq_factor`` divided by ``factor``, blended between
+      yarn             by pair index: kept above ``beta_fast`` (32) turns, divided below ``beta_slow`` (1), a ramp between;
+                       attention_scale = ``attention_factor``, else 0.1 ln(factor) + 1
+    """
+    dim = int(model_config.head_dim * (getattr(model_config, "partial_rotary_factor", 1.0) or 1.0))
+    dim -= dim % 2
+    if dim < 2:
+        raise ValueError("the rotated part of a head has at least two elements")
+    base = float(getattr(model_config, "rope_theta", 10000.0) or 10000.0)
+    scaling = getattr(model_config, "rope_scaling", None)
+    if scaling is None:
+        scaling = {}
+    elif isinstance(scaling, (int, float)):
+        scaling = {"rope_type": "linear", "factor": float(scaling)}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    factor = float(scaling.get("factor", 1.0))
+    if kind not in ("default", "linear", "ntk", "llama3", "yarn"):
+        raise ValueError(f"unknown rope_type {kind!r}")
+    if kind != "default" and not factor > 0:
+        raise ValueError("the scaling factor is positive")
+    if kind == "ntk" and dim > 2:
+        base *= factor ** (dim / (dim - 2))
+    inv = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    attention_scale = 1.0
+    if kind == "linear":
+        inv = inv / factor
+    elif kind in ("llama3", "yarn"):
+        original = scaling.get("original_max_position_embeddings") or getattr(model_config, "max_position_embeddings", None)
+        if not original:
+            raise ValueError(f"{kind} scaling needs original_max_position_embeddings")
+        if kind == "llama3":
+            low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+            if not high > low:
+                raise ValueError("high_freq_factor is above low_freq_factor")
+            keep = ((original * inv / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+            inv = inv * keep + inv / factor * (1 - keep)
+        else:
+            at = [dim * math.log(original / (float(scaling.get(name, turns)) * 2 * math.pi)) / (2 * math.log(base))
+                  for name, turns in (("beta_fast", 32.0), ("beta_slow", 1.0))]
+            low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dim - 1)
+            ramp = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+            inv = inv / factor * ramp + inv * (1 - ramp)
+            attention_scale = scaling.get("attention_factor")
+            if attention_scale is None:
+                attention_scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    return inv.to(device), float(attention_scale)
+
+
+def rotary_embedding_positions(
+    q: torch.Tensor,                # [num_tokens, num_q_heads, head_dim]
+    k: torch.Tensor,                # [num_tokens, num_kv_heads, head_dim]
+    positions: torch.Tensor,        # [num_tokens] int32 or int64
+    inv_freq: torch.Tensor,         # [rotary_dim / 2] float64, radians a position (see rotary_inv_freq)
+    *,
+    interleaved: bool = False,      # pairs are neighbours (2j, 2j + 1) instead of (j, j + rotary_dim / 2)
+    attention_scale: float = 1.0,
+    q_out: torch.Tensor = None,     # where the result goes; default: in place
+    k_out: torch.Tensor = None,
+):
+    """Rotate pair j of every head of token t by ``positions[t] * inv_freq[j]`` and scale it by ``attention_scale``;
+    elements behind the rotated part pass through unchanged.  In place, or into ``q_out`` / ``k_out`` (memory that does
+    not overlap q and k).  fp16, bf16 or fp32, computed in fp32 and rounded once.  Elements are contiguous; tokens and
+    heads may lie any distance apart, so q and k may be views of one fused projection.  Any position that a 64-bit float
+    holds keeps its angle to about 2^-24 of half a turn."""
+    require_cuda(q, "q")
+    q_out = q if q_out is None else q_out
+    k_out = k if k_out is None else k_out
+    device, n = q.device, q.shape[0]
+    for t in (q, k, q_out, k_out):
+        assert t.dim() == 3 and t.shape[0] == n and t.dtype == q.dtype and t.device == device
+        assert t.stride(2) == 1 and t.shape[2] == q.shape[2], "elements are contiguous, one head_dim"
+        assert t.shape[0] <= 1 or t.stride(0) >= t.shape[2], "tokens do not overlap"
+        assert t.shape[1] <= 1 or t.stride(1) >= t.shape[2], "heads do not overlap"
+    assert q_out.shape == q.shape and k_out.shape == k.shape
+    code = _DTYPES.get(q.dtype)
+    if code is None:
+        raise RuntimeError(f"unsupported dtype {q.dtype}")
+    assert positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous() and positions.shape == (n,)
+    assert inv_freq.dtype == torch.float64 and inv_freq.is_contiguous() and inv_freq.dim() == 1
+    assert positions.device == device and inv_freq.device == device
+    assert 2 * inv_freq.shape[0] <= q.shape[2], "inv_freq has at most head_dim / 2 entries"
+    dev, stream = device_and_stream(q)
+    strides = (C.c_int64 * 8)(q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                              q_out.stride(0), q_out.stride(1), k_out.stride(0), k_out.stride(1))
+    check(lib.mkv_rotary_positions(
+        dev, stream, q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), strides, positions.data_ptr(),
+        positions.element_size(), inv_freq.data_ptr(), inv_freq.shape[0], bool(interleaved), attention_scale, n,
+        q.shape[1], k.shape[1], q.shape[2], code), "mkv_rotary_positions")
