@@ -99,12 +99,13 @@ __global__ void attn_q8_plain_kernel(const T *__restrict__ q, int64_t q_stride, 
 }
 
 // ------------------------------------------------------------------ fast kernel
-constexpr int kTileTokens = 16;
-constexpr int kUnitCost = 2;      // phantom tiles in front of a (sequence, head)
-constexpr int kMinTiles = 8;      // ... least number of tiles a thread block is started for
+constexpr int kHalf = 16;         // tokens of a tensor-core tile
+constexpr int kTile = 32;         // tokens of a tile: two of those, so that a loop pass has enough to do
+constexpr int kUnitCost = 1;      // phantom tiles in front of a (sequence, head)
+constexpr int kMinTiles = 8;      // least number of positions a thread block is started for
 constexpr float kBoost = 6.f;     // weights are held as 2^(score - max + 6): fp16 then reaches 2^-20 of the largest in full
 constexpr float kLag = 4.f;       // the running maximum follows only when a score is above it by 2^4
-constexpr float kScaleRange = 16.f;  // block scales within this factor of the piece's first go into the weights
+constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
@@ -123,10 +124,15 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ uint2 lds8(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// Four 8 x 8 matrices of 16-bit elements, transposed: thread (g, t) gets elements (2t, g) and (2t + 1, g) of each.
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -146,22 +152,46 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
+}
 
-// Four codes (one word) as two half2, exact.  int8: the byte with its sign bit flipped is q + 128; set behind the byte 0x64 it
-// is the fp16 number 1024 + 128 + q.
+// int8 codes as fp16: the byte with its sign bit flipped is q + 128; set behind the byte 0x64 it is the fp16 number
+// 1024 + 128 + q.  K keeps the offset - the score's accumulator starts at -1152 sum(q) instead of 0, which costs at most
+// 1152 sum|q| 2^-22 in a score, less than summing 128 products in 32 bits may - while V's is taken off: a sum of weights
+// over a long context would bury the result under it.
+constexpr float kCodeOffset = 1152.f;
+
+// K: codes (0, 1) and (2, 3) of a word.
 template <int CODE>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t &lo, uint32_t &hi) {
+__device__ __forceinline__ void widen_k(uint32_t w, uint32_t &lo, uint32_t &hi) {
     if (CODE == MKV_Q8_INT8) {
         const uint32_t x = w ^ 0x80808080u;
-        const __half2 off = __float2half2_rn(-1152.f);
-        lo = half2_bits(__hadd2(bits_half2(__byte_perm(x, 0x64646464u, 0x4140)), off));
-        hi = half2_bits(__hadd2(bits_half2(__byte_perm(x, 0x64646464u, 0x4342)), off));
+        lo = __byte_perm(x, 0x64646464u, 0x4140);
+        hi = __byte_perm(x, 0x64646464u, 0x4342);
     } else {
-        lo = e4m3x2_to_half2(w & 0xffffu);
-        hi = e4m3x2_to_half2(w >> 16);
+        e4m3x4_to_half2(w, lo, hi);
+    }
+}
+// V: codes (0, 2) and (1, 3) of a word: two tokens of one dim, then of the next.
+template <int CODE>
+__device__ __forceinline__ void widen_v(uint32_t w, uint32_t &even, uint32_t &odd) {
+    if (CODE == MKV_Q8_INT8) {
+        const uint32_t x = w ^ 0x80808080u;
+        const __half2 off = __float2half2_rn(-kCodeOffset);
+        even = half2_bits(__hadd2(bits_half2(__byte_perm(x, 0x64646464u, 0x4240)), off));
+        odd = half2_bits(__hadd2(bits_half2(__byte_perm(x, 0x64646464u, 0x4341)), off));
+    } else {
+        e4m3x4_to_half2(__byte_perm(w, 0u, 0x3120), even, odd);
     }
 }
 
+template <typename T>
+__device__ __forceinline__ void store2(T *dst, float a, float b) {
+    struct alignas(2 * sizeof(T)) Two { T x[2]; } v;
+    v.x[0] = rounded<T>(a); v.x[1] = rounded<T>(b);
+    *reinterpret_cast<Two *>(dst) = v;
+}
 template <typename T>
 __device__ __forceinline__ void store4(T *dst, float a, float b, float c, float d) {
     struct alignas(8) Four { T x[4]; } v;
@@ -178,8 +208,9 @@ struct AttnQ8Params {
     int64_t table_cols;
     int num_rows;
     const int32_t *seq_ids, *seq_lens;
-    int batch, num_q_heads, group, groups;  // groups: units of up to 8 * NT query heads for each kv head
-    int cur_layer, tile_shift;              // tiles of a block: 1 << tile_shift
+    int batch, num_q_heads, group, groups;  // groups: units of up to HC query heads for each kv head
+    int cur_layer, half_shift;              // halves (16 tokens) of a block: 1 << half_shift
+    int max_len;                            // tokens that a row of the table can hold
     float scale_log2;
     int *error_flags, *arrive;
     float *head_rows, *block_rows;          // [worker] and [2 * block] rows of HC * D values + HC log-sums
@@ -189,7 +220,7 @@ struct Piece {      // a (sequence, head) that a warp has some tiles of
     int b, hp;      // batch index; kv head * groups + head group
     int flags;      // 1 valid, 2 has the first tile, 4 has the last tile, 8 parked in the ring (else in the warp's row)
     int nt;         // tiles of the whole (sequence, head)
-    long long p0;   // where it starts in the launch's order
+    long long p0;   // where its first real tile stands in the launch's order
 };
 
 // First position of thread block c's range.
@@ -200,12 +231,13 @@ __device__ __forceinline__ int range_owner(long long x, long long T, int R) { re
 template <typename T, int CODE, int D, int NT, bool DUP, int WARPS, int STAGES, int BLOCKS>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __grid_constant__ AttnQ8Params p) {
     constexpr int HC = DUP ? 4 : 8 * NT;        // query heads of a unit
-    constexpr int TILE = kTileTokens * D;       // bytes of K (or V)
-    constexpr int STAGE = 2 * TILE + 48;        // K, V, and: K scale, V scale, b, hp, flags, tokens, tile, tiles, start
+    constexpr int HB = kHalf * D;               // bytes of K (or V) of a half
+    constexpr int META = 4 * HB;                // scales (K, K, V, V) | flags and tokens, tile, -, - | b, hp, tiles, positions left
+    constexpr int STAGE = META + 48;            // K, K, V, V, and those
     constexpr int KW = D / 16;                  // words of K a thread takes from a token's row = k-steps
-    constexpr int VW = D / 32;                  // words of V a thread takes from a token's row
     constexpr int MT = D / 16;                  // row tiles of O^T
     constexpr int ROW = HC * D + HC;            // floats of a partial row
+    constexpr bool kScaledQ = !std::is_same<T, __half>::value;
     static_assert(STAGES * STAGE >= ROW * 4, "a piece is parked in its warp's ring");
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Piece first_piece[WARPS], last_piece[WARPS];
@@ -219,8 +251,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     const uint32_t ring = smem_addr(ring_ptr);
 
     // ---- this block's range ---------------------------------------------------------------------------------
-    const long long most_tiles = p.table_cols << p.tile_shift;  // what a row of the table can hold
-    auto tiles_of = [&](int len) { return len <= 0 ? 0 : (int)min(((long long)len + kTileTokens - 1) / kTileTokens, most_tiles); };
+    auto tiles_of = [&](int len) { return len <= 0 ? 0 : (int)(((unsigned)min(len, p.max_len) + kTile - 1) / kTile); };
     const int per = (p.batch + WARPS * 32 - 1) / (WARPS * 32);
     long long mine = 0;
     for (int i = 0; i < per; ++i) {
@@ -265,51 +296,62 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     __syncthreads();
     const long long wlo = lo + (hi - lo) * warp / WARPS, whi = lo + (hi - lo) * (warp + 1) / WARPS;
 
-    // ---- where the warp reads next (all of this is the same in every lane, the windows apart) ---------------------
-    bool bad = false;
-    int cb = 0, chp = 0, ch = 0, chg = 0, cnt = 0, cj = 0, cjend = 0, clen = 0, crow = 0, cbase = 0;
-    long long cp0 = 0;
-    bool more = false, cfirst = true;
-    int wb = 0, wlen = 0, wrow = 0;         // lane l: length and table row of sequence wb + l
-    int ids = 0, ids_next = 0, ids0 = 0, ids0_next = 0;  // block ids of 32 tiles: at cbase, behind it, at tile 0 of this
-                                                         // sequence and of the next
-    auto load_window = [&](int b) {
-        wb = b;
-        wlen = b + lane < p.batch ? __ldg(p.seq_lens + b + lane) : 0;
-        wrow = b + lane < p.batch ? __ldg(p.seq_ids + b + lane) : 0;
-    };
+    // ---- where the warp reads next: the same in every lane, the id windows apart -----------------------------------
+    // crem: positions from the current (sequence, head)'s first real tile to the end of the warp's range, whose part of it
+    // therefore ends at min(cnt, crem).
+    const int half_mask = (1 << p.half_shift) - 1;
+    bool bad = false, more = false;
+    int cb = 0, chp = 0, ch = 0, chg = 0, cnt = 0, cj = 0, cjend = 0, clen = 0, crow = 0, cbase = 0, crem = 0;
+    int first_flag = 1;
+    int64_t uoff = 0;               // bytes of the unit's (layer, head) inside a block's codes
+    int2 ids, ids_next;             // lane l: block ids of tile cbase + l's halves, and of the 32 tiles behind those
+    int2 ids0_next = make_int2(-1, -1);  // ... of the first 32 tiles of the next sequence (nb; its row and length)
+    int nb = -1, nrow = 0, nlen = 0;
     auto load_ids = [&](int row, int first, int nt) {
         const int tile = first + lane;
-        if (row < 0 || row >= p.num_rows || tile >= nt) return -1;
-        return __ldg(p.block_table + (int64_t)row * p.table_cols + (tile >> p.tile_shift));
-    };
-    // first sequence behind cb that has tokens: its window lane is found by a vote; -1: none
-    auto next_sequence = [&]() {
-        int at = cb + 1;
-        while (at < p.batch) {
-            if (at >= wb + 32) load_window(at);
-            const unsigned some = __ballot_sync(0xffffffffu, wlen > 0) & (0xffffffffu << (at - wb));
-            if (some) return wb + __ffs(some) - 1;
-            at = wb + 32;
+        int2 x = make_int2(-1, -1);
+        if (row >= 0 && row < p.num_rows && tile < nt) {
+            const int32_t *at = p.block_table + (int64_t)row * p.table_cols;
+            const int a = (2 * tile) >> p.half_shift, b = (2 * tile + 1) >> p.half_shift;
+            x.x = __ldg(at + a);
+            if (b < p.table_cols) x.y = __ldg(at + b);
         }
-        return -1;
+        return x;
     };
-    int nb = -1, nrow = 0, nlen = 0;        // the next sequence
-    auto look_ahead = [&]() {
-        nb = next_sequence();
-        if (nb >= 0) {
-            nrow = __shfl_sync(0xffffffffu, wrow, nb - wb);
-            nlen = __shfl_sync(0xffffffffu, wlen, nb - wb);
-            ids0_next = load_ids(nrow, 0, tiles_of(nlen));
+    auto look_ahead = [&]() {   // the first sequence behind cb that has tokens
+        nb = -1;
+        for (int at = cb + 1; at < p.batch; at += 32) {
+            const int len = at + lane < p.batch ? __ldg(p.seq_lens + at + lane) : 0;
+            const unsigned some = __ballot_sync(0xffffffffu, len > 0);
+            if (some) {
+                nb = at + __ffs(some) - 1;
+                nlen = __shfl_sync(0xffffffffu, len, __ffs(some) - 1);
+                nrow = __ldg(p.seq_ids + nb);
+                ids0_next = load_ids(nrow, 0, tiles_of(nlen));
+                return;
+            }
         }
+    };
+    auto enter_sequence = [&]() {
+        cnt = tiles_of(clen);
+        bad |= crow < 0 || crow >= p.num_rows || clen > p.max_len;
+        clen = min(clen, p.max_len);
+    };
+    auto enter_head = [&]() {
+        uoff = (int64_t)(p.cur_layer * p.pool.num_kv_heads + ch) * p.pool.tile_bytes;
+        cjend = min(cnt, crem);
+        more = cj < cjend;
+        cbase = cj;
+        first_flag = 1;
+        if (more) ids_next = load_ids(crow, cj + 32, cnt);
     };
     if (wlo < whi) {
         // the sequence that holds position wlo
         long long at = start_pos[warp];
         int b = start_b[warp];
         while (b < p.batch) {
-            load_window(b);
-            const int nt = tiles_of(wlen);
+            const int len = b + lane < p.batch ? __ldg(p.seq_lens + b + lane) : 0;
+            const int nt = tiles_of(len);
             const long long w = nt > 0 ? (long long)(nt + kUnitCost) * P : 0;
             long long sum = w;
 #pragma unroll
@@ -322,137 +364,145 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 const int src = __ffs(here) - 1;
                 cb = b + src;
                 at += __shfl_sync(0xffffffffu, sum - w, src);
-                clen = __shfl_sync(0xffffffffu, wlen, src);
-                crow = __shfl_sync(0xffffffffu, wrow, src);
+                clen = __shfl_sync(0xffffffffu, len, src);
+                crow = __ldg(p.seq_ids + cb);
                 break;
             }
             at += __shfl_sync(0xffffffffu, sum, 31);
             b += 32;
         }
-        cnt = tiles_of(clen);
+        enter_sequence();
         const int w = cnt + kUnitCost;
         const long long rem = wlo - at;
         chp = (int)min(rem / w, (long long)P - 1);
-        cp0 = at + (long long)chp * w;
-        cj = max((int)(wlo - cp0) - kUnitCost, 0);
+        const int inside = (int)(rem - (long long)chp * w);
+        cj = max(inside - kUnitCost, 0);
+        crem = (int)(whi - wlo) + inside - kUnitCost;
         ch = chp / p.groups;
         chg = chp - ch * p.groups;
-        cjend = (int)min((long long)cnt, whi - cp0 - kUnitCost);
-        more = cj < cjend;
-        if (more) {
-            cbase = cj;
-            ids = load_ids(crow, cj, cnt);
-            ids_next = load_ids(crow, cj + 32, cnt);
-            ids0 = load_ids(crow, 0, cnt);
-            look_ahead();
-            bad |= crow < 0 || crow >= p.num_rows || (long long)cnt * kTileTokens < clen;
-        }
+        ids = load_ids(crow, cj, cnt);
+        enter_head();
+        if (more) look_ahead();
     }
-    // One tile into ring stage `slot`, and the cursor moves on.
-    int issued = 0;
-    auto issue = [&](int slot) {
+    const uint64_t lane16 = (uint64_t)lane * 16;
+    const uint32_t block_tiles = (uint32_t)(p.pool.num_layers * p.pool.num_kv_heads);
+    const uint32_t block_bytes = (uint32_t)p.pool.tile_bytes * block_tiles;
+    // 16-byte piece i * 32 + lane of a half.  D = 128: piece c of token r goes to c ^ (r & 7); D = 64: two tokens share a
+    // 128-byte line, whose pieces go to c ^ (line & 3).  Either way the reads below meet no conflict.
+    const uint32_t put = (uint32_t)((lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
+    auto issue_half = [&](uint32_t st, int h, uint32_t blk, int &tokens) {
+        if (tokens > 0 && blk < (uint64_t)p.pool.total_blocks) {
+            int seg = 0;
+            uint32_t row = blk;
+            if (p.pool.num_segments > 1) {
+                int64_t r;
+                locate_block(p.pool, blk, seg, r);
+                row = (uint32_t)r;
+            }
+            const uint64_t off = (uint64_t)row * block_bytes + uoff + (uint32_t)(((2 * cj + h) & half_mask) * HB) + lane16;
+            const uint8_t *kt = p.pool.k_base[seg] + off, *vt = p.pool.v_base[seg] + off;
+#pragma unroll
+            for (int i = 0; i < HB / 512; ++i) {
+                const uint32_t to = st + h * HB + i * 512 + (D == 128 && (i & 1) ? put ^ 64 : put);
+                cp16(to, kt + i * 512);
+                cp16(to + 2 * HB, vt + i * 512);
+            }
+            if (lane < 2)
+                cp4(st + META + (lane * 2 + h) * 4, (lane ? p.pool.v_scale[seg] : p.pool.k_scale[seg]) +
+                                                        ((uint64_t)row * block_tiles + p.cur_layer * p.pool.num_kv_heads + ch));
+        } else {
+            bad |= tokens > 0;
+            tokens = 0;
+            if (lane < 2) asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(st + META + (lane * 2 + h) * 4), "r"(0x3f800000) : "memory");
+        }
+    };
+    // One tile into ring stage `st`, and the cursor moves on.
+    auto issue = [&](uint32_t st) {
         if (!more) return;
         if (cj - cbase == 32) {
             ids = ids_next;
-            cbase += 32;
+            cbase = cj;
             ids_next = load_ids(crow, cbase + 32, cnt);
         }
-        const int blk = __shfl_sync(0xffffffffu, ids, cj - cbase);
-        const uint32_t st = ring + slot * STAGE;
-        int tokens = min(kTileTokens, clen - cj * kTileTokens);
-        if (blk >= 0 && blk < p.pool.total_blocks) {
-            int seg = 0;
-            int64_t row = blk;
-            if (p.pool.num_segments > 1) locate_block(p.pool, blk, seg, row);
-            const int64_t tile = tile_index(p.pool, row, p.cur_layer, ch);
-            const int64_t off = ((tile << p.tile_shift) + (cj & ((1 << p.tile_shift) - 1))) * TILE;
-            const uint8_t *kt = p.pool.k_base[seg] + off, *vt = p.pool.v_base[seg] + off;
-#pragma unroll
-            for (int i = 0; i < TILE / 512; ++i) {
-                // 16-byte piece `id` of the tile; D = 128: piece c of token r goes to c ^ (r & 7); D = 64: two tokens share a
-                // 128-byte line, whose pieces go to c ^ (line & 3) * 2.  Either way the reads below meet no conflict.
-                const int id = i * 32 + lane, line = id >> 3, c = id & 7;
-                const uint32_t to = line * 128 + ((c ^ (D == 128 ? line & 7 : (line & 3) * 2)) << 4);
-                cp16(st + to, kt + id * 16);
-                cp16(st + TILE + to, vt + id * 16);
-            }
-            if (lane < 2) cp4(st + 2 * TILE + lane * 4, (lane ? p.pool.v_scale[seg] : p.pool.k_scale[seg]) + tile);
-        } else {
-            tokens = 0;
-            bad = true;
-        }
-        const bool last = cj + 1 == cjend;
-        if (lane == 0) {
-            const int flags = (cfirst ? 1 : 0) | (last ? 2 : 0);
-            asm volatile("st.shared.v2.b32 [%0], {%1,%2};\n" ::"r"(st + 2 * TILE + 8), "r"(cb), "r"(chp) : "memory");
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(st + 2 * TILE + 16), "r"(flags), "r"(tokens), "r"(cj), "r"(cnt) : "memory");
-            asm volatile("st.shared.b64 [%0], %1;\n" ::"r"(st + 2 * TILE + 32), "l"(cp0) : "memory");
-        }
-        ++issued;
-        cfirst = false;
-        ++cj;
-        if (last) {     // the next (sequence, head)
-            cfirst = true;
-            cp0 += cnt + kUnitCost;
-            if (++chp == P) {
-                if (nb < 0) {
-                    more = false;
-                    return;
+        const uint32_t blk0 = (uint32_t)__shfl_sync(0xffffffffu, ids.x, cj - cbase);
+        const uint32_t blk1 = (uint32_t)__shfl_sync(0xffffffffu, ids.y, cj - cbase);
+        const int left = clen - cj * kTile;
+        int n0 = min(left, kHalf), n1 = min(max(left - kHalf, 0), kHalf);
+        issue_half(st, 0, blk0, n0);
+        issue_half(st, 1, blk1, n1);
+        int flags = first_flag;
+        first_flag = 0;
+        const int tile = cj++;
+        const int b = cb, hp = chp, nt = cnt, end = crem;
+        if (cj == cjend) {      // the next (sequence, head)
+            flags |= 2;
+            crem -= cnt + kUnitCost;
+            if (crem <= 0) {
+                more = false;
+            } else if (++chp == P) {
+                more = false;
+                if (nb >= 0) {
+                    cb = nb;
+                    crow = nrow;
+                    clen = nlen;
+                    ids = ids0_next;
+                    chp = ch = chg = cj = 0;
+                    enter_sequence();
+                    enter_head();
+                    if (more) look_ahead();
                 }
-                cb = nb;
-                crow = nrow;
-                clen = nlen;
-                cnt = tiles_of(clen);
-                chp = ch = chg = 0;
-                ids0 = ids0_next;
-                look_ahead();
-                bad |= crow < 0 || crow >= p.num_rows || (long long)cnt * kTileTokens < clen;
-            } else if (++chg == p.groups) {
-                chg = 0;
-                ++ch;
+            } else {
+                if (++chg == p.groups) {
+                    chg = 0;
+                    ++ch;
+                }
+                cj = 0;
+                ids = load_ids(crow, 0, cnt);   // the row was read for the head before: an L1 hit
+                enter_head();
             }
-            cj = cbase = 0;
-            cjend = (int)min((long long)cnt, whi - cp0 - kUnitCost);
-            more = cjend > 0;
-            ids = ids0;
-            if (more) ids_next = load_ids(crow, 32, cnt);
+            if (!more) flags |= 4;
+        }
+        if (lane == 0) {
+            sts16(st + META + 16, flags | (n0 << 8) | (n1 << 16), tile, 0, 0);
+            if (flags & 3) sts16(st + META + 32, b, hp, nt, end);
         }
     };
 
     float o[NT][MT][4];
     uint32_t qf[NT][KW][2];
-    float qfac[NT][2];       // scale_log2 and what undoes the normalisation of q, for heads 2t and 2t + 1
+    float qfac[NT][2];      // scale_log2 and what undoes the normalisation of a bf16 q, for heads 2t and 2t + 1
+    float kinit[NT][2];     // what takes the offset of int8 codes out of the scores
     float thr[NT][2], base[NT][2], l[NT][2];
-    float vref = 0.f, vinv = 0.f;
-    int piece_starts = 0;
+    bool piece_starts = false;
+    // byte offsets inside a half: K pieces of tokens g and g + 8; V rows and pieces for ldmatrix
+    const uint32_t k_at = D == 128 ? g * 128 + (((2 * t) ^ g) << 4) : (g >> 1) * 128 + ((((g & 1) * 4 + t) ^ (g >> 1)) << 4);
+    const int vr = (lane & 7) + ((lane >> 3) & 1) * 8, vh = lane >> 4;
+    const uint32_t v_at = 2 * HB + (D == 128 ? vr * 128 + ((vh ^ (vr & 7)) << 4)
+                                             : (vr >> 1) * 128 + ((((vr & 1) * 4 + vh) ^ ((vr >> 1) & 3)) << 4));
 
+    bool busy = more;
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        issue(s);
+    for (int i = 0; i < STAGES - 1; ++i) {
+        issue(ring + i * STAGE);
         cp_commit();
     }
-    int slot = 0, done = 0;
-    while (done < issued) {
+    uint32_t st = ring, refill = ring + (STAGES - 1) * STAGE;
+    while (busy) {
         cp_wait<STAGES - 2>();
         __syncwarp();       // every lane's part of the tile has landed, and the stage before it is read
-        issue(slot == 0 ? STAGES - 1 : slot - 1);
+        issue(refill);
         cp_commit();
-        const uint32_t st = ring + slot * STAGE;
-        ++done;
-        slot = slot + 1 == STAGES ? 0 : slot + 1;
-        const uint4 ma = lds16(st + 2 * TILE), mb = lds16(st + 2 * TILE + 16);
-        const float ks = __uint_as_float(ma.x), vs = __uint_as_float(ma.y);
-        const int b = (int)ma.z, hp = (int)ma.w, flags = (int)mb.x, tokens = (int)mb.y;
-        int hq0 = 0, heads = 0;     // query heads of the unit
-        if (flags & 3) {
-            const int kvh = hp / p.groups;
-            hq0 = kvh * p.group + (hp - kvh * p.groups) * HC;
-            heads = min(HC, (kvh + 1) * p.group - hq0);
-        }
+        const uint4 scales = lds16(st + META), ma = lds16(st + META + 16);
+        const int flags = (int)(ma.x & 0xffu);
+        const int tokens[2] = {(int)((ma.x >> 8) & 0xffu), (int)(ma.x >> 16)};
+        busy = !(flags & 4);
 
         if (flags & 1) {    // first tile of a piece
-            piece_starts = mb.z == 0;
-            const T *qb = (const T *)p.q + b * p.q_stride + (int64_t)hq0 * D + t * (D / 4);
+            piece_starts = ma.y == 0;
+            const uint4 mb = lds16(st + META + 32);
+            const int kvh = (int)mb.y / p.groups, hq0 = kvh * p.group + ((int)mb.y - kvh * p.groups) * HC;
+            const int heads = min(HC, (kvh + 1) * p.group - hq0);
+            const T *qb = (const T *)p.q + (int)mb.x * p.q_stride + (int64_t)hq0 * D + t * (D / 4);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 // column g of the tile is query head g (DUP: g & 3, so that columns 4-7 repeat 0-3); this thread holds its
@@ -465,8 +515,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     if (head < heads) x = __ldg(reinterpret_cast<const uint4 *>(qb + (int64_t)head * D) + i);
                     raw[4 * i] = x.x; raw[4 * i + 1] = x.y; raw[4 * i + 2] = x.z; raw[4 * i + 3] = x.w;
                 }
-                float fac = p.scale_log2;
-                if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+                if (kScaledQ) {
                     // bf16: a power of two brings the head's largest element to [2^14, 2^15); then fp16 holds every element
                     // down to 2^-28 of it exactly
                     uint32_t peak = 0;
@@ -476,177 +525,170 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
                     const int e = peak == 0 ? 0 : min(max(14 + 127 - (int)(peak >> 7), -120), 120);
                     const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-                    fac *= __uint_as_float((uint32_t)(127 - e) << 23);
+                    const float fac = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
                     for (int i = 0; i < KW * 2; ++i)
                         raw[i] = half2_bits(__floats2half2_rn(__uint_as_float(raw[i] << 16) * up, __uint_as_float(raw[i] & 0xffff0000u) * up));
+                    // columns 2t and 2t + 1 belong to the lanes with g = 2t and 2t + 1
+                    qfac[n][0] = __shfl_sync(0xffffffffu, fac, 8 * t);
+                    qfac[n][1] = __shfl_sync(0xffffffffu, fac, 8 * t + 4);
+                }
+                if (CODE == MKV_Q8_INT8) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < KW * 2; ++i) {
+                        const float2 f = __half22float2(bits_half2(raw[i]));
+                        sum += f.x + f.y;
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    kinit[n][0] = -kCodeOffset * __shfl_sync(0xffffffffu, sum, 8 * t);
+                    kinit[n][1] = -kCodeOffset * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
                 }
 #pragma unroll
                 for (int i = 0; i < KW; ++i) {
                     qf[n][i][0] = raw[2 * i];
                     qf[n][i][1] = raw[2 * i + 1];
                 }
-                // columns 2t and 2t + 1 belong to the lanes with g = 2t and 2t + 1
-                qfac[n][0] = __shfl_sync(0xffffffffu, fac, 8 * t);
-                qfac[n][1] = __shfl_sync(0xffffffffu, fac, 8 * t + 4);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
                 thr[n][0] = thr[n][1] = -INFINITY;
                 base[n][0] = base[n][1] = l[n][0] = l[n][1] = 0.f;
             }
-            vref = 0.f;
         }
 
-        if (tokens > 0) {
-            // ---- S^T = K Q^T
-            float sc[NT][2][4];
+        // ---- S^T = K Q^T
+        float sc[2][NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float part[NT][2][4];   // two chains, for the latency
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[n][0][e] = sc[n][1][e] = 0.f;
-            {
-                uint32_t lo8[KW], hi8[KW];      // words of tokens g and g + 8
-                if constexpr (D == 128) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t at = st + g * 128 + (((2 * t + i) ^ g) << 4);
-                        const uint4 x = lds16(at), y = lds16(at + 1024);
-                        lo8[4 * i] = x.x; lo8[4 * i + 1] = x.y; lo8[4 * i + 2] = x.z; lo8[4 * i + 3] = x.w;
-                        hi8[4 * i] = y.x; hi8[4 * i + 1] = y.y; hi8[4 * i + 2] = y.z; hi8[4 * i + 3] = y.w;
-                    }
-                } else {
-                    const int line = g >> 1;
-                    const uint32_t at = st + line * 128 + (((((g & 1) << 2) + t) ^ (line * 2)) << 4);
-                    const uint4 x = lds16(at), y = lds16(at + 512);
-                    lo8[0] = x.x; lo8[1] = x.y; lo8[2] = x.z; lo8[3] = x.w;
-                    hi8[0] = y.x; hi8[1] = y.y; hi8[2] = y.z; hi8[3] = y.w;
+                for (int e = 0; e < 4; ++e) {
+                    part[n][0][e] = CODE == MKV_Q8_INT8 ? kinit[n][e & 1] : 0.f;
+                    part[n][1][e] = 0.f;
                 }
 #pragma unroll
-                for (int i = 0; i < KW; ++i) {
+            for (int i = 0; i < KW / 4; ++i) {
+                const uint32_t at = st + h * HB + (k_at ^ (i << 4));
+                const uint4 x = lds16(at), y = lds16(at + HB / 2);      // tokens g and g + 8
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
                     uint32_t a0, a1, a2, a3;
-                    widen<CODE>(lo8[i], a0, a2);
-                    widen<CODE>(hi8[i], a1, a3);
+                    widen_k<CODE>(xs[j], a0, a2);
+                    widen_k<CODE>(ys[j], a1, a3);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma(sc[n][i & 1], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+                    for (int n = 0; n < NT; ++n) mma(part[n][j & 1], a0, a1, a2, a3, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
                 }
             }
-            // ---- softmax: token g (elements 0, 1) and g + 8 (2, 3) of heads 2t, 2t + 1
-            const bool on0 = g < tokens, on1 = g + 8 < tokens;
-            float s0[NT][4];
-            bool above = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[h][n][e] = part[n][0][e] + part[n][1][e];
+        }
+        // ---- softmax: token g (elements 0, 1) and g + 8 (2, 3) of each half, heads 2t, 2t + 1
+        // The block's V scale joins the exponent: weights are 2^(score + log2 s_v - base), so that O accumulates across
+        // blocks as the tensor core leaves it, and the denominator takes them back over s_v.  A scale below 2^-100 (an
+        // all-zero block's, above all) counts as 2^-100, and does not move the maximum.
+        float iv[2];
+        bool above = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float ks = __uint_as_float(h ? scales.y : scales.x), vs = __uint_as_float(h ? scales.w : scales.z);
+            const float sv = vs < kLeastScale ? kLeastScale : vs;
+            float lv;
+            asm("lg2.approx.f32 %0, %1;\n" : "=f"(lv) : "f"(sv));
+            asm("rcp.approx.f32 %0, %1;\n" : "=f"(iv[h]) : "f"(sv));
+            const bool on0 = g < tokens[h], on1 = g + 8 < tokens[h];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float f0 = qfac[n][0] * ks, f1 = qfac[n][1] * ks;
-                s0[n][0] = on0 ? (sc[n][0][0] + sc[n][1][0]) * f0 : -INFINITY;
-                s0[n][1] = on0 ? (sc[n][0][1] + sc[n][1][1]) * f1 : -INFINITY;
-                s0[n][2] = on1 ? (sc[n][0][2] + sc[n][1][2]) * f0 : -INFINITY;
-                s0[n][3] = on1 ? (sc[n][0][3] + sc[n][1][3]) * f1 : -INFINITY;
-                above |= fmaxf(s0[n][0], s0[n][2]) > thr[n][0] || fmaxf(s0[n][1], s0[n][3]) > thr[n][1];
+                const float f0 = (kScaledQ ? qfac[n][0] : p.scale_log2) * ks, f1 = (kScaledQ ? qfac[n][1] : p.scale_log2) * ks;
+                sc[h][n][0] = on0 ? fmaf(sc[h][n][0], f0, lv) : -INFINITY;
+                sc[h][n][1] = on0 ? fmaf(sc[h][n][1], f1, lv) : -INFINITY;
+                sc[h][n][2] = on1 ? fmaf(sc[h][n][2], f0, lv) : -INFINITY;
+                sc[h][n][3] = on1 ? fmaf(sc[h][n][3], f1, lv) : -INFINITY;
             }
-            if (__any_sync(0xffffffffu, above)) {   // the maxima settle after the first tiles of a piece
+        }
+        float mx[NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float m = fmaxf(s0[n][e], s0[n][e + 2]);
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                        m = fmaxf(m, thr[n][e] - kLag);
-                        const float nb = m == -INFINITY ? 0.f : m - kBoost;
-                        const float a = thr[n][e] == -INFINITY ? 1.f : ex2(base[n][e] - nb);   // before: all weights were 0
-                        thr[n][e] = m + kLag;
-                        base[n][e] = nb;
-                        l[n][e] *= a;
+            for (int e = 0; e < 2; ++e) {
+                mx[n][e] = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
+                above |= mx[n][e] > thr[n][e];
+            }
+        if (__any_sync(0xffffffffu, above)) {   // the maxima settle after the first tiles of a piece
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            o[n][i][e] *= a;
-                            o[n][i][e + 2] *= a;
-                        }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float m = mx[n][e];
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    m = fmaxf(m, thr[n][e] - kLag);
+                    const float to = m == -INFINITY ? 0.f : m - kBoost;
+                    const float a = thr[n][e] == -INFINITY ? 1.f : ex2(base[n][e] - to);   // before: all weights were 0
+                    thr[n][e] = m + kLag;
+                    base[n][e] = to;
+                    l[n][e] *= a;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        o[n][i][e] *= a;
+                        o[n][i][e + 2] *= a;
                     }
-            }
-            // The block's V scale goes into the weights while it is near the piece's first one, otherwise the block's
-            // product is scaled on its own.
-            if (vref == 0.f) {
-                vref = vs > 0.f ? vs : 1.f;
-                vinv = 1.f / vref;
-            }
-            const float ratio = vs * vinv;
-            const bool near_ref = ratio <= kScaleRange && ratio >= 1.f / kScaleRange;
-            const float wr = near_ref ? ratio : 1.f;
-            uint32_t pb[NT][2];
+                }
+        }
+        uint32_t pb[2][NT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float w0 = ex2(s0[n][0] - base[n][0]), w1 = ex2(s0[n][1] - base[n][1]);
-                const float w2 = ex2(s0[n][2] - base[n][0]), w3 = ex2(s0[n][3] - base[n][1]);
-                l[n][0] += w0 + w2;
-                l[n][1] += w1 + w3;
-                __half2 x = __floats2half2_rn(w0 * wr, w1 * wr), y = __floats2half2_rn(w2 * wr, w3 * wr);
+                const float w0 = ex2(sc[h][n][0] - base[n][0]), w1 = ex2(sc[h][n][1] - base[n][1]);
+                const float w2 = ex2(sc[h][n][2] - base[n][0]), w3 = ex2(sc[h][n][3] - base[n][1]);
+                l[n][0] = fmaf(w0 + w2, iv[h], l[n][0]);
+                l[n][1] = fmaf(w1 + w3, iv[h], l[n][1]);
+                __half2 x = __floats2half2_rn(w0, w1), y = __floats2half2_rn(w2, w3);
                 if (DUP) {  // columns 4-7: what the rounding of columns 0-3 left over
                     const float2 fx = __half22float2(x), fy = __half22float2(y);
-                    const __half2 rx = __floats2half2_rn(w0 * wr - fx.x, w1 * wr - fx.y);
-                    const __half2 ry = __floats2half2_rn(w2 * wr - fy.x, w3 * wr - fy.y);
-                    if (t >= 2) {
-                        x = rx;
-                        y = ry;
-                    }
+                    const __half2 rx = __floats2half2_rn(w0 - fx.x, w1 - fx.y), ry = __floats2half2_rn(w2 - fy.x, w3 - fy.y);
+                    x = t >= 2 ? rx : x;
+                    y = t >= 2 ? ry : y;
                 }
-                pb[n][0] = transpose8x8(half2_bits(x));
-                pb[n][1] = transpose8x8(half2_bits(y));
+                pb[h][n][0] = transpose8x8(half2_bits(x));
+                pb[h][n][1] = transpose8x8(half2_bits(y));
             }
-            // ---- O^T += V^T P^T: row tile i has dim (D / 8) g + i in its row g and dim (D / 8) g + MT + i in its row g + 8
-            uint32_t vw[4][VW];     // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+        // ---- O^T += V^T P^T: row tile c has dim 16 c + 2 g in its row g and dim 16 c + 2 g + 1 in its row g + 8
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int tok = 2 * t + (k & 1) + (k >> 1) * 8;
-                if constexpr (D == 128) {
-                    const uint4 x = lds16(st + TILE + tok * 128 + ((g ^ (tok & 7)) << 4));
-                    vw[k][0] = x.x; vw[k][1] = x.y; vw[k][2] = x.z; vw[k][3] = x.w;
-                } else {
-                    const int line = tok >> 1;
-                    const uint2 x = lds8(st + TILE + line * 128 + (((((tok & 1) << 2) + (g >> 1)) ^ ((line & 3) * 2)) << 4) + (g & 1) * 8);
-                    vw[k][0] = x.x; vw[k][1] = x.y;
-                }
-                if (CODE == MKV_Q8_E4M3 && tokens < kTileTokens && tok >= tokens) {
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int c = 0; c < MT; c += 2) {
+                uint32_t w[4];      // (16-dim piece c: tokens 0-7, 8-15; piece c + 1: the same)
+                ldsm4_trans(w, st + h * HB + (v_at ^ (c << 4)));
+                if (CODE == MKV_Q8_E4M3 && tokens[h] < kHalf) {
                     // behind the sequence's end any byte may stand, NaN among them, and 0 x NaN is NaN
-#pragma unroll
-                    for (int i = 0; i < VW; ++i) vw[k][i] = 0u;
+                    const int n = tokens[h] - 2 * t;
+                    const uint32_t lo = n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u, hi = n >= 10 ? 0xffffffffu : n == 9 ? 0xffffu : 0u;
+                    w[0] &= lo; w[1] &= hi; w[2] &= lo; w[3] &= hi;
                 }
-            }
-            auto fragments = [&](int i, uint32_t (&x)[4], uint32_t (&y)[4]) {
-                // words i: dims 4i ... 4i + 3 of this thread's; x[d]: (token 2t, token 2t + 1), y[d]: tokens 2t + 8, 2t + 9
-                widen<CODE>(__byte_perm(vw[0][i], vw[1][i], 0x5140), x[0], x[1]);
-                widen<CODE>(__byte_perm(vw[0][i], vw[1][i], 0x7362), x[2], x[3]);
-                widen<CODE>(__byte_perm(vw[2][i], vw[3][i], 0x5140), y[0], y[1]);
-                widen<CODE>(__byte_perm(vw[2][i], vw[3][i], 0x7362), y[2], y[3]);
-            };
 #pragma unroll
-            for (int i = 0; i < VW / 2; ++i) {
-                uint32_t xa[4], ya[4], xb[4], yb[4];
-                fragments(i, xa, ya);               // dims 4i + d
-                fragments(i + VW / 2, xb, yb);      // dims MT + 4i + d
-                if (near_ref) {
+                for (int d = 0; d < 2; ++d) {
+                    uint32_t a0, a1, a2, a3;
+                    widen_v<CODE>(w[2 * d], a0, a1);
+                    widen_v<CODE>(w[2 * d + 1], a2, a3);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma(o[n][4 * i + d], xa[d], xb[d], ya[d], yb[d], pb[n][0], pb[n][1]);
-                } else {
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float part[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma(part, xa[d], xb[d], ya[d], yb[d], pb[n][0], pb[n][1]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[n][4 * i + d][e] = fmaf(part[e], ratio, o[n][4 * i + d][e]);
-                        }
+                    for (int n = 0; n < NT; ++n) mma(o[n][c + d], a0, a1, a2, a3, pb[h][n][0], pb[h][n][1]);
                 }
             }
         }
 
         if (flags & 2) {    // last tile of the piece
-            const bool ends = (int)mb.z + 1 == (int)mb.w, whole = piece_starts && ends, final_piece = done == issued;
-            const float vr = vref == 0.f ? 1.f : vref;
+            const uint4 mb = lds16(st + META + 32);
+            const int b = (int)mb.x, kvh = (int)mb.y / p.groups, hq0 = kvh * p.group + ((int)mb.y - kvh * p.groups) * HC;
+            const int heads = min(HC, (kvh + 1) * p.group - hq0);
+            const bool ends = ma.y + 1 == mb.z, whole = piece_starts && ends;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -664,17 +706,16 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
             }
             float *row = nullptr;
             if (!whole) {
-                Piece &pc = final_piece && first_piece[warp].flags ? last_piece[warp] : first_piece[warp];
-                // (a piece that is neither first nor last of its warp is whole)
-                row = final_piece ? reinterpret_cast<float *>(ring_ptr)
-                                  : p.head_rows + ((int64_t)cta * WARPS + warp) * ROW;
+                // (a piece that is neither the first nor the last of its warp is whole)
+                Piece &pc = !busy && first_piece[warp].flags ? last_piece[warp] : first_piece[warp];
+                row = busy ? p.head_rows + ((int64_t)cta * WARPS + warp) * ROW : reinterpret_cast<float *>(ring_ptr);
                 __syncwarp();
                 if (lane == 0) {
                     pc.b = b;
-                    pc.hp = hp;
-                    pc.nt = (int)mb.w;
-                    pc.flags = 1 | (piece_starts ? 2 : 0) | (ends ? 4 : 0) | (final_piece ? 8 : 0);
-                    asm volatile("ld.shared.b64 %0, [%1];\n" : "=l"(pc.p0) : "r"(st + 2 * TILE + 32) : "memory");
+                    pc.hp = (int)mb.y;
+                    pc.nt = (int)mb.z;
+                    pc.flags = 1 | (piece_starts ? 2 : 0) | (ends ? 4 : 0) | (busy ? 0 : 8);
+                    pc.p0 = whi - (int)mb.w;
                 }
                 __syncwarp();
             }
@@ -685,26 +726,22 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     const int head = n * 8 + 2 * t + e;
                     if (head >= heads || head >= HC) continue;
                     if (whole) {
-                        const float f = vr / l[n][e];
-                        T *dst = (T *)p.o + ((int64_t)b * p.num_q_heads + hq0 + head) * D + g * (D / 8);
+                        const float f = 1.f / l[n][e];
+                        T *dst = (T *)p.o + ((int64_t)b * p.num_q_heads + hq0 + head) * D + 2 * g;
 #pragma unroll
-                        for (int i = 0; i < MT; i += 4) {
-                            store4<T>(dst + i, o[n][i][e] * f, o[n][i + 1][e] * f, o[n][i + 2][e] * f, o[n][i + 3][e] * f);
-                            store4<T>(dst + MT + i, o[n][i][e + 2] * f, o[n][i + 1][e + 2] * f, o[n][i + 2][e + 2] * f, o[n][i + 3][e + 2] * f);
-                        }
+                        for (int i = 0; i < MT; ++i) store2<T>(dst + 16 * i, o[n][i][e] * f, o[n][i][e + 2] * f);
                     } else {
-                        const float f = l[n][e] == 0.f ? 0.f : vr / l[n][e];
-                        float *dst = row + head * D + g * (D / 8);
+                        const float f = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+                        float *dst = row + head * D + 2 * g;
 #pragma unroll
-                        for (int i = 0; i < MT; i += 4) {
-                            *reinterpret_cast<float4 *>(dst + i) = make_float4(o[n][i][e] * f, o[n][i + 1][e] * f, o[n][i + 2][e] * f, o[n][i + 3][e] * f);
-                            *reinterpret_cast<float4 *>(dst + MT + i) =
-                                make_float4(o[n][i][e + 2] * f, o[n][i + 1][e + 2] * f, o[n][i + 2][e + 2] * f, o[n][i + 3][e + 2] * f);
-                        }
+                        for (int i = 0; i < MT; ++i)
+                            *reinterpret_cast<float2 *>(dst + 16 * i) = make_float2(o[n][i][e] * f, o[n][i][e + 2] * f);
                         if (g == 0) row[HC * D + head] = log2f(l[n][e]) + base[n][e];
                     }
                 }
         }
+        refill = st;
+        st = st == ring + (STAGES - 1) * STAGE ? ring : st + STAGE;
     }
     cp_wait<0>();
     if (bad && lane == 0 && p.error_flags) atomicOr(p.error_flags, 1);
@@ -758,9 +795,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 if (lane == 0) {
                     __stcg(row + HC * D + r, log2f(sum) + (m == -INFINITY ? 0.f : m));
                     if (r == 0) {
-                        const long long at = lead.p0 + kUnitCost;
-                        cross_f[s] = range_owner(at, total, R);
-                        cross_n[s] = range_owner(at + lead.nt - 1, total, R) - cross_f[s] + 1;
+                        cross_f[s] = range_owner(lead.p0, total, R);
+                        cross_n[s] = range_owner(lead.p0 + lead.nt - 1, total, R) - cross_f[s] + 1;
                         cross_b[s] = lead.b;
                         cross_hp[s] = lead.hp;
                         cross_valid[s] = 1;
@@ -824,19 +860,18 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
 
 // ------------------------------------------------------------------ host side
 constexpr int kWarps = 8;
-constexpr int kMaxBlocksPerSm = 2;
+constexpr int kBlocksPerSm = 1;
 constexpr size_t kErrorBytes = 256;     // error word, then the arrival counters
 
-static size_t zero_bytes(int sms) { return kErrorBytes + (((size_t)sms * kMaxBlocksPerSm * sizeof(int) + 255) & ~(size_t)255); }
+static size_t zero_bytes(int sms) { return kErrorBytes + (((size_t)sms * kBlocksPerSm * sizeof(int) + 255) & ~(size_t)255); }
 // Query heads of a unit: 4 (columns 4-7 of the tile then carry what fp16 loses of the weights), 8 or 16.
 static int unit_heads(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
-static int blocks_per_sm(int heads) { return heads == 16 ? 1 : 2; }
 
-static bool fast_shape(int group, int head_dim, int block_size) {
-    (void)group;
-    return (head_dim == 64 || head_dim == 128) && block_size >= 16 && (block_size & (block_size - 1)) == 0;
+static bool fast_shape(const PoolViewQ8 &pv) {
+    const int bs = pv.block_size;
+    return (pv.head_dim == 64 || pv.head_dim == 128) && bs >= kHalf && (bs & (bs - 1)) == 0 &&
+           pv.tile_bytes * pv.num_layers * pv.num_kv_heads < (1ll << 32) && pv.total_blocks < (1ll << 31);
 }
-
 // 16-byte loads of q and of the pool, 8-byte stores of o.
 static bool fast_aligned(const PoolViewQ8 &pv, const void *q, int64_t q_stride, const void *o) {
     uintptr_t bits = (uintptr_t)q | (uintptr_t)(q_stride * 2) | ((uintptr_t)o << 1);
@@ -844,10 +879,10 @@ static bool fast_aligned(const PoolViewQ8 &pv, const void *q, int64_t q_stride, 
     return (bits & 15) == 0;
 }
 
-template <typename T, int CODE, int D, int NT, bool DUP, int STAGES, int BLOCKS>
+template <typename T, int CODE, int D, int NT, bool DUP, int STAGES>
 static cudaError_t launch_fast(const AttnQ8Params &p, unsigned grid, cudaStream_t s) {
-    constexpr int smem = kWarps * STAGES * (2 * kTileTokens * D + 48);
-    auto kernel = attn_q8_kernel<T, CODE, D, NT, DUP, kWarps, STAGES, BLOCKS>;
+    constexpr int smem = kWarps * STAGES * (4 * kHalf * D + 48);
+    auto kernel = attn_q8_kernel<T, CODE, D, NT, DUP, kWarps, STAGES, kBlocksPerSm>;
     static std::atomic<bool> configured[64];    // per device; setting the attribute twice is harmless
     int dev = 0;
     cudaGetDevice(&dev);
@@ -864,12 +899,12 @@ template <typename T, int CODE>
 static cudaError_t launch_fast_shape(const AttnQ8Params &p, int head_dim, unsigned grid, cudaStream_t s) {
     const int heads = unit_heads(p.group);
     if (head_dim == 128)
-        return heads == 4   ? launch_fast<T, CODE, 128, 1, true, 3, 2>(p, grid, s)
-               : heads == 8 ? launch_fast<T, CODE, 128, 1, false, 3, 2>(p, grid, s)
-                            : launch_fast<T, CODE, 128, 2, false, 6, 1>(p, grid, s);
-    return heads == 4   ? launch_fast<T, CODE, 64, 1, true, 6, 2>(p, grid, s)
-           : heads == 8 ? launch_fast<T, CODE, 64, 1, false, 6, 2>(p, grid, s)
-                        : launch_fast<T, CODE, 64, 2, false, 8, 1>(p, grid, s);
+        return heads == 4   ? launch_fast<T, CODE, 128, 1, true, 3>(p, grid, s)
+               : heads == 8 ? launch_fast<T, CODE, 128, 1, false, 3>(p, grid, s)
+                            : launch_fast<T, CODE, 128, 2, false, 3>(p, grid, s);
+    return heads == 4   ? launch_fast<T, CODE, 64, 1, true, 5>(p, grid, s)
+           : heads == 8 ? launch_fast<T, CODE, 64, 1, false, 5>(p, grid, s)
+                        : launch_fast<T, CODE, 64, 2, false, 5>(p, grid, s);
 }
 
 }  // namespace mkv
@@ -887,7 +922,7 @@ size_t mkv_attn_q8_workspace_bytes(int device, int batch, int num_q_heads, int n
     int sms = 0;
     if (batch < 0 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1 || mkv_sm_count(device, &sms) != MKV_OK) return 0;
     const int heads = unit_heads(num_q_heads / num_kv_heads);
-    const size_t rows = (size_t)sms * blocks_per_sm(heads) * (kWarps + 2);
+    const size_t rows = (size_t)sms * kBlocksPerSm * (kWarps + 2);
     return zero_bytes(sms) + rows * heads * (head_dim + 1) * sizeof(float);
 }
 
@@ -913,7 +948,7 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
     int *flags = workspace && workspace_bytes >= kErrorBytes ? (int *)workspace : nullptr;
     const float scale_log2 = softmax_scale * kLog2e;
     const int group = num_q_heads / pv.num_kv_heads;
-    if (dtype != MKV_F32 && fast_shape(group, pv.head_dim, pv.block_size) && fast_aligned(pv, q, q_stride, o)) {
+    if (dtype != MKV_F32 && fast_shape(pv) && fast_aligned(pv, q, q_stride, o)) {
         int sms = 0;
         if ((st = mkv_sm_count(device, &sms))) return st;
         if (!workspace || workspace_bytes < mkv_attn_q8_workspace_bytes(device, batch, num_q_heads, pv.num_kv_heads, pv.head_dim))
@@ -934,11 +969,12 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
         p.group = group;
         p.groups = (group + heads - 1) / heads;
         p.cur_layer = cur_layer;
-        p.tile_shift = 0;
-        while ((kTileTokens << p.tile_shift) < pv.block_size) ++p.tile_shift;
+        p.half_shift = 0;
+        while ((kHalf << p.half_shift) < pv.block_size) ++p.half_shift;
+        p.max_len = (int)std::min<int64_t>(table_stride * pv.block_size, 0x7fffffff);
         p.scale_log2 = scale_log2;
-        const int most = sms * blocks_per_sm(heads);
-        const int64_t positions = (int64_t)batch * (ceil_div64(max_seq_len, kTileTokens) + kUnitCost) * pv.num_kv_heads * p.groups;
+        const int most = sms * kBlocksPerSm;
+        const int64_t positions = (int64_t)batch * (ceil_div64(max_seq_len, kTile) + kUnitCost) * pv.num_kv_heads * p.groups;
         const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, positions / kMinTiles));
         p.error_flags = (int *)workspace;
         p.arrive = (int *)((char *)workspace + kErrorBytes);
