@@ -102,7 +102,6 @@ __global__ void attn_q8_plain_kernel(const T *__restrict__ q, int64_t q_stride, 
 constexpr int kHalf = 16;         // tokens of a tensor-core tile
 constexpr int kTile = 32;         // tokens of a tile: two of those, so that a loop pass has enough to do
 constexpr int kUnitCost = 1;      // phantom tiles in front of a (sequence, head)
-constexpr int kMinTiles = 8;      // least number of positions a thread block is started for
 constexpr float kBoost = 6.f;     // weights are held as 2^(score - max + 6): fp16 then reaches 2^-20 of the largest in full
 constexpr float kLag = 4.f;       // the running maximum follows only when a score is above it by 2^4
 constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
@@ -278,7 +277,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         if (w < warp) before += scan_w[w];
         total += scan_w[w];
     }
-    const int R = (int)max(1ll, min((long long)gridDim.x, total / kMinTiles));
+    // (a position at least for each warp of a block: a piece that enters a block is then its first warp's)
+    const int R = (int)max(1ll, min((long long)gridDim.x, total / WARPS));
     const int cta = blockIdx.x;
     if (total == 0 || cta >= R) return;
     const long long lo = range_start(cta, total, R), hi = range_start(cta + 1, total, R);
@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kWarps = 8;
+constexpr int kWarps = 12, kWarpsWide = 8;  // warps of a block; with 16 query heads a unit, whose accumulators take more registers
 constexpr int kBlocksPerSm = 1;
 constexpr size_t kErrorBytes = 256;     // error word, then the arrival counters
 
@@ -881,8 +881,9 @@ static bool fast_aligned(const PoolViewQ8 &pv, const void *q, int64_t q_stride, 
 
 template <typename T, int CODE, int D, int NT, bool DUP, int STAGES>
 static cudaError_t launch_fast(const AttnQ8Params &p, unsigned grid, cudaStream_t s) {
-    constexpr int smem = kWarps * STAGES * (4 * kHalf * D + 48);
-    auto kernel = attn_q8_kernel<T, CODE, D, NT, DUP, kWarps, STAGES, kBlocksPerSm>;
+    constexpr int warps = NT == 2 ? kWarpsWide : kWarps;
+    constexpr int smem = warps * STAGES * (4 * kHalf * D + 48);
+    auto kernel = attn_q8_kernel<T, CODE, D, NT, DUP, warps, STAGES, kBlocksPerSm>;
     static std::atomic<bool> configured[64];    // per device; setting the attribute twice is harmless
     int dev = 0;
     cudaGetDevice(&dev);
@@ -891,7 +892,7 @@ static cudaError_t launch_fast(const AttnQ8Params &p, unsigned grid, cudaStream_
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
     }
-    kernel<<<grid, kWarps * 32, smem, s>>>(p);
+    kernel<<<grid, warps * 32, smem, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -899,11 +900,11 @@ template <typename T, int CODE>
 static cudaError_t launch_fast_shape(const AttnQ8Params &p, int head_dim, unsigned grid, cudaStream_t s) {
     const int heads = unit_heads(p.group);
     if (head_dim == 128)
-        return heads == 4   ? launch_fast<T, CODE, 128, 1, true, 3>(p, grid, s)
-               : heads == 8 ? launch_fast<T, CODE, 128, 1, false, 3>(p, grid, s)
+        return heads == 4   ? launch_fast<T, CODE, 128, 1, true, 2>(p, grid, s)
+               : heads == 8 ? launch_fast<T, CODE, 128, 1, false, 2>(p, grid, s)
                             : launch_fast<T, CODE, 128, 2, false, 3>(p, grid, s);
-    return heads == 4   ? launch_fast<T, CODE, 64, 1, true, 5>(p, grid, s)
-           : heads == 8 ? launch_fast<T, CODE, 64, 1, false, 5>(p, grid, s)
+    return heads == 4   ? launch_fast<T, CODE, 64, 1, true, 4>(p, grid, s)
+           : heads == 8 ? launch_fast<T, CODE, 64, 1, false, 4>(p, grid, s)
                         : launch_fast<T, CODE, 64, 2, false, 5>(p, grid, s);
 }
 
@@ -975,7 +976,7 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
         p.scale_log2 = scale_log2;
         const int most = sms * kBlocksPerSm;
         const int64_t positions = (int64_t)batch * (ceil_div64(max_seq_len, kTile) + kUnitCost) * pv.num_kv_heads * p.groups;
-        const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, positions / kMinTiles));
+        const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, positions / (heads == 16 ? kWarpsWide : kWarps)));
         p.error_flags = (int *)workspace;
         p.arrive = (int *)((char *)workspace + kErrorBytes);
         p.head_rows = (float *)((char *)workspace + zero_bytes(sms));
