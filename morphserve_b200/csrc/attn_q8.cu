@@ -101,7 +101,7 @@ __global__ void attn_q8_plain_kernel(const T *__restrict__ q, int64_t q_stride, 
 // ------------------------------------------------------------------ fast kernel
 constexpr int kHalf = 16;         // tokens of a tensor-core tile
 constexpr int kTile = 32;         // tokens of a tile: two of those, so that a loop pass has enough to do
-constexpr int kUnitCost = 1;      // phantom tiles in front of a (sequence, head)
+constexpr int kUnitCost = 2;      // phantom tiles in front of a (sequence, head)
 constexpr float kBoost = 6.f;     // weights are held as 2^(score - max + 6): fp16 then reaches 2^-20 of the largest in full
 constexpr float kLag = 4.f;       // the running maximum follows only when a score is above it by 2^4
 constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
@@ -219,13 +219,19 @@ struct Piece {      // a (sequence, head) that a warp has some tiles of
     int b, hp;      // batch index; kv head * groups + head group
     int flags;      // 1 valid, 2 has the first tile, 4 has the last tile, 8 parked in the ring (else in the warp's row)
     int nt;         // tiles of the whole (sequence, head)
-    long long p0;   // where its first real tile stands in the launch's order
+    int p0;         // where its first real tile stands in the launch's order
 };
 
-// First position of thread block c's range.
-__device__ __forceinline__ long long range_start(int c, long long T, int R) { return (long long)c * T / R; }
-// Thread block whose range holds position x.
-__device__ __forceinline__ int range_owner(long long x, long long T, int R) { return (int)(((x + 1) * R - 1) / T); }
+// `total` positions in n contiguous shares, whose sizes differ by one at most.
+struct Shares {
+    int n, size, more;      // the first `more` shares have size + 1
+    __device__ __forceinline__ Shares(int total, int n_) : n(n_), size(total / n_), more(total - size * n_) {}
+    __device__ __forceinline__ int start(int i) const { return i * size + min(i, more); }
+    __device__ __forceinline__ int owner(int x) const {
+        const int big = more * (size + 1);
+        return x < big ? x / (size + 1) : more + (x - big) / max(size, 1);
+    }
+};
 
 template <typename T, int CODE, int D, int NT, bool DUP, int WARPS, int STAGES, int BLOCKS>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __grid_constant__ AttnQ8Params p) {
@@ -240,8 +246,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     static_assert(STAGES * STAGE >= ROW * 4, "a piece is parked in its warp's ring");
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Piece first_piece[WARPS], last_piece[WARPS];
-    __shared__ long long scan_w[WARPS], start_pos[WARPS];
-    __shared__ int start_b[WARPS];
+    __shared__ int scan_w[WARPS];
+    __shared__ int4 start_at[WARPS];    // where a warp's range starts: batch index, its first position, length, table row
     __shared__ int cross_valid[2], cross_f[2], cross_n[2], cross_b[2], cross_hp[2], cross_last[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -251,50 +257,61 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
 
     // ---- this block's range ---------------------------------------------------------------------------------
     auto tiles_of = [&](int len) { return len <= 0 ? 0 : (int)(((unsigned)min(len, p.max_len) + kTile - 1) / kTile); };
+    // Thread i counts the positions of sequences [i per, (i + 1) per).
     const int per = (p.batch + WARPS * 32 - 1) / (WARPS * 32);
-    long long mine = 0;
+    int mine = 0, my_len = 0, my_row = 0;
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
         if (b < p.batch) {
-            const int nt = tiles_of(p.seq_lens[b]);
+            my_len = __ldg(p.seq_lens + b);
+            my_row = __ldg(p.seq_ids + b);      // (used if there is one sequence a thread: fetched along with the length)
+            const int nt = tiles_of(my_len);
             if (nt > 0) mine += nt + kUnitCost;
         }
     }
     mine *= P;
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long n = __shfl_up_sync(0xffffffffu, incl, d);
+        const int n = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += n;
     }
     if (lane == 31) scan_w[warp] = incl;
     if (lane == 0) first_piece[warp].flags = last_piece[warp].flags = 0;
     if (tid < 2) cross_valid[tid] = cross_last[tid] = 0;
     __syncthreads();
-    long long total = 0, before = 0;
+    int total = 0, from = incl - mine;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) before += scan_w[w];
+        if (w < warp) from += scan_w[w];
         total += scan_w[w];
     }
-    // (a position at least for each warp of a block: a piece that enters a block is then its first warp's)
-    const int R = (int)max(1ll, min((long long)gridDim.x, total / WARPS));
+    // A position at least for each warp of a block, so that a piece that enters a block is its first warp's.
+    const Shares blocks(total, max(min((int)gridDim.x, total / WARPS), 1));
     const int cta = blockIdx.x;
-    if (total == 0 || cta >= R) return;
-    const long long lo = range_start(cta, total, R), hi = range_start(cta + 1, total, R);
-    {
-        const long long from = before + incl - mine;
-#pragma unroll
+    if (total == 0 || cta >= blocks.n) return;
+    const int lo = blocks.start(cta), hi = blocks.start(cta + 1);
+    const Shares warps(hi - lo, WARPS);
+    if (mine > 0 && from < hi && from + mine > lo) {
+#pragma unroll 1
         for (int w = 0; w < WARPS; ++w) {
-            const long long x = lo + (hi - lo) * w / WARPS;
-            if (x >= from && x < from + mine) {
-                start_b[w] = tid * per;
-                start_pos[w] = from;
+            const int x = lo + warps.start(w);
+            if (x < from || x >= from + mine) continue;
+            int b = tid * per, at = from, len = my_len, row = my_row;
+            if (per > 1) {
+                for (;; ++b) {      // (one of them holds x)
+                    len = __ldg(p.seq_lens + b);
+                    const int nt = tiles_of(len), c = nt > 0 ? (nt + kUnitCost) * P : 0;
+                    if (x < at + c || b + 1 == min((tid + 1) * per, p.batch)) break;
+                    at += c;
+                }
+                row = __ldg(p.seq_ids + b);
             }
+            start_at[w] = make_int4(b, at, len, row);
         }
     }
     __syncthreads();
-    const long long wlo = lo + (hi - lo) * warp / WARPS, whi = lo + (hi - lo) * (warp + 1) / WARPS;
+    const int wlo = lo + warps.start(warp), whi = lo + warps.start(warp + 1);
 
     // ---- where the warp reads next: the same in every lane, the id windows apart -----------------------------------
     // crem: positions from the current (sequence, head)'s first real tile to the end of the warp's range, whose part of it
@@ -306,7 +323,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     int64_t uoff = 0;               // bytes of the unit's (layer, head) inside a block's codes
     int2 ids, ids_next;             // lane l: block ids of tile cbase + l's halves, and of the 32 tiles behind those
     int2 ids0_next = make_int2(-1, -1);  // ... of the first 32 tiles of the next sequence (nb; its row and length)
-    int nb = -1, nrow = 0, nlen = 0;
+    int nb = -2, nrow = 0, nlen = 0;    // -1: there is none, -2: not looked for yet
     auto load_ids = [&](int row, int first, int nt) {
         const int tile = first + lane;
         int2 x = make_int2(-1, -1);
@@ -346,43 +363,20 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         if (more) ids_next = load_ids(crow, cj + 32, cnt);
     };
     if (wlo < whi) {
-        // the sequence that holds position wlo
-        long long at = start_pos[warp];
-        int b = start_b[warp];
-        while (b < p.batch) {
-            const int len = b + lane < p.batch ? __ldg(p.seq_lens + b + lane) : 0;
-            const int nt = tiles_of(len);
-            const long long w = nt > 0 ? (long long)(nt + kUnitCost) * P : 0;
-            long long sum = w;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const long long n = __shfl_up_sync(0xffffffffu, sum, d);
-                if (lane >= d) sum += n;
-            }
-            const unsigned here = __ballot_sync(0xffffffffu, wlo < at + sum);
-            if (here) {
-                const int src = __ffs(here) - 1;
-                cb = b + src;
-                at += __shfl_sync(0xffffffffu, sum - w, src);
-                clen = __shfl_sync(0xffffffffu, len, src);
-                crow = __ldg(p.seq_ids + cb);
-                break;
-            }
-            at += __shfl_sync(0xffffffffu, sum, 31);
-            b += 32;
-        }
+        const int4 at = start_at[warp];
+        cb = at.x;
+        clen = at.z;
+        crow = at.w;
         enter_sequence();
-        const int w = cnt + kUnitCost;
-        const long long rem = wlo - at;
-        chp = (int)min(rem / w, (long long)P - 1);
-        const int inside = (int)(rem - (long long)chp * w);
+        const unsigned w = cnt + kUnitCost, rem = wlo - at.y;
+        chp = min((int)(rem / w), P - 1);
+        const int inside = (int)(rem - chp * w);
         cj = max(inside - kUnitCost, 0);
-        crem = (int)(whi - wlo) + inside - kUnitCost;
+        crem = whi - wlo + inside - kUnitCost;
         ch = chp / p.groups;
         chg = chp - ch * p.groups;
         ids = load_ids(crow, cj, cnt);
         enter_head();
-        if (more) look_ahead();
     }
     const uint64_t lane16 = (uint64_t)lane * 16;
     const uint32_t block_tiles = (uint32_t)(p.pool.num_layers * p.pool.num_kv_heads);
@@ -430,6 +424,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         int n0 = min(left, kHalf), n1 = min(max(left - kHalf, 0), kHalf);
         issue_half(st, 0, blk0, n0);
         issue_half(st, 1, blk1, n1);
+        if (first_flag) {       // the unit's query rows on their way into the cache
+            const int hq0 = ch * p.group + chg * HC, bytes = min(HC, p.group - chg * HC) * D * 2;
+            if (lane * 128 < bytes)
+                asm volatile("prefetch.global.L1 [%0];\n" ::"l"((const char *)((const T *)p.q + cb * p.q_stride + (int64_t)hq0 * D) + lane * 128));
+        }
         int flags = first_flag;
         first_flag = 0;
         const int tile = cj++;
@@ -441,15 +440,16 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 more = false;
             } else if (++chp == P) {
                 more = false;
+                if (nb == -2) look_ahead();
                 if (nb >= 0) {
                     cb = nb;
                     crow = nrow;
                     clen = nlen;
                     ids = ids0_next;
                     chp = ch = chg = cj = 0;
+                    nb = -2;
                     enter_sequence();
                     enter_head();
-                    if (more) look_ahead();
                 }
             } else {
                 if (++chg == p.groups) {
@@ -492,6 +492,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         __syncwarp();       // every lane's part of the tile has landed, and the stage before it is read
         issue(refill);
         cp_commit();
+        if (more && nb == -2) look_ahead();     // early, so that the next sequence's ids are there when it comes
         const uint4 scales = lds16(st + META), ma = lds16(st + META + 16);
         const int flags = (int)(ma.x & 0xffu);
         const int tokens[2] = {(int)((ma.x >> 8) & 0xffu), (int)(ma.x >> 16)};
@@ -746,65 +747,120 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     cp_wait<0>();
     if (bad && lane == 0 && p.error_flags) atomicOr(p.error_flags, 1);
 
-    // ---- pieces of cut (sequence, head)s: those of this block's warps are folded, one warp for each query head -----------
+    // ---- pieces of cut (sequence, head)s: those of this block's warps are folded, four query heads by one warp -----------
     __syncthreads();
-    bool leads = false;     // lane c: the first or last piece of warp c / 2 is the block's first piece of its (sequence, head)
-    if (lane < 2 * WARPS) {
-        const int fl = ((lane & 1) ? last_piece[lane >> 1] : first_piece[lane >> 1]).flags;
-        leads = fl != 0 && ((fl & 2) != 0 || lane == 0);
+    // Lane c: is the first (c even) or last (odd) piece of warp c / 2 the block's first one of its (sequence, head)?  Its
+    // others are the first pieces of the warps behind it, up to the one that ends.
+    unsigned leaders, held, ending;
+    {
+        const int fl = lane < 2 * WARPS ? ((lane & 1) ? last_piece[lane >> 1] : first_piece[lane >> 1]).flags : 0;
+        leaders = __ballot_sync(0xffffffffu, fl != 0 && ((fl & 2) != 0 || lane == 0));
+        const int ff = lane < WARPS ? first_piece[lane].flags : 0;
+        held = __ballot_sync(0xffffffffu, ff != 0);
+        ending = __ballot_sync(0xffffffffu, (ff & 4) != 0);
     }
-    unsigned leaders = __ballot_sync(0xffffffffu, leads);
+    constexpr int QUADS = (HC + 3) / 4;
+    const unsigned all_leaders = leaders;
     int item = 0;
-    while (leaders) {
-        const int c = __ffs(leaders) - 1;
-        leaders &= leaders - 1;
-        const Piece lead = (c & 1) ? last_piece[c >> 1] : first_piece[c >> 1];
-        const int kvh = lead.hp / p.groups, hq0 = kvh * p.group + (lead.hp - kvh * p.groups) * HC;
-        const int heads = min(HC, (kvh + 1) * p.group - hq0);
-        for (int r = 0; r < heads; ++r) {
+#pragma unroll 1
+    for (; leaders; leaders &= leaders - 1) {
+        const int c = __ffs(leaders) - 1, x0 = c >> 1;
+#pragma unroll 1
+        for (int quad = 0; quad < QUADS; ++quad) {
             if (item++ % WARPS != warp) continue;
-            float m = -INFINITY, sum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            int x = c >> 1, fl = lead.flags;
-            for (;;) {
-                const float *row = (fl & 8) ? reinterpret_cast<const float *>(smem + x * (STAGES * STAGE))
-                                            : p.head_rows + ((int64_t)cta * WARPS + x) * ROW;
-                const float ls = row[HC * D + r];
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (lane * 4 < D) v = *reinterpret_cast<const float4 *>(row + r * D + lane * 4);
-                const float nm = fmaxf(m, ls), off = nm == -INFINITY ? 0.f : nm;
-                const float a = exp2f(m - off), e = exp2f(ls - off);
-                acc.x = acc.x * a + v.x * e; acc.y = acc.y * a + v.y * e; acc.z = acc.z * a + v.z * e; acc.w = acc.w * a + v.w * e;
-                sum = sum * a + e;
-                m = nm;
-                if (fl & 4) break;
-                do ++x; while (x < WARPS && first_piece[x].flags == 0);
-                if (x == WARPS) break;
-                fl = first_piece[x].flags;
+            const Piece lead = (c & 1) ? last_piece[x0] : first_piece[x0];
+            const int kvh = lead.hp / p.groups, hq0 = kvh * p.group + (lead.hp - kvh * p.groups) * HC;
+            const int heads = min(HC, (kvh + 1) * p.group - hq0) - quad * 4;
+            if (heads <= 0) continue;
+            unsigned behind = 0;        // warps that hold the further pieces
+            bool ends = lead.flags & 4;
+            if (!ends) {
+                behind = held & ~((2u << x0) - 1);
+                const unsigned e = behind & ending;
+                ends = e != 0;
+                if (ends) behind &= (e & (0u - e)) * 2 - 1;
             }
-            if ((lead.flags & 2) && (fl & 4)) {     // all of it lies in this block
-                const float f = 1.f / sum;
-                if (lane * 4 < D)
-                    store4<T>((T *)p.o + ((int64_t)lead.b * p.num_q_heads + hq0 + r) * D + lane * 4, acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-            } else {
-                // row 0 of the block: of a (sequence, head) that comes from the block before it; row 1: of one that starts here
-                const int s = (lead.flags & 2) ? 1 : 0;
-                float *row = p.block_rows + ((int64_t)cta * 2 + s) * ROW;
-                const float f = sum == 0.f ? 0.f : 1.f / sum;
-                if (lane * 4 < D) __stcg(reinterpret_cast<float4 *>(row + r * D + lane * 4), make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-                if (lane == 0) {
-                    __stcg(row + HC * D + r, log2f(sum) + (m == -INFINITY ? 0.f : m));
-                    if (r == 0) {
-                        cross_f[s] = range_owner(lead.p0, total, R);
-                        cross_n[s] = range_owner(lead.p0 + lead.nt - 1, total, R) - cross_f[s] + 1;
-                        cross_b[s] = lead.b;
-                        cross_hp[s] = lead.hp;
-                        cross_valid[s] = 1;
+            float m[4], sum[4];
+            float4 acc[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                m[r] = -INFINITY;
+                sum[r] = 0.f;
+                acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            int x[2] = {x0, 0}, fl[2] = {lead.flags, 0};
+            int n = 1;
+            for (;;) {
+                if (n == 1 && behind) {     // two pieces at a time: all loads before the first use
+                    x[1] = __ffs(behind) - 1;
+                    behind &= behind - 1;
+                    fl[1] = first_piece[x[1]].flags;
+                    n = 2;
+                }
+                float ls[2][4];
+                float4 v[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float *row = (fl[i] & 8) ? reinterpret_cast<const float *>(smem + x[i] * (STAGES * STAGE))
+                                                   : p.head_rows + ((int64_t)cta * WARPS + x[i]) * ROW;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int head = quad * 4 + min(r, heads - 1);
+                        ls[i][r] = -INFINITY;
+                        v[i][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (i < n) {
+                            ls[i][r] = row[HC * D + head];
+                            if (lane * 4 < D) v[i][r] = *reinterpret_cast<const float4 *>(row + head * D + lane * 4);
+                        }
                     }
                 }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float nm = fmaxf(m[r], fmaxf(ls[0][r], ls[1][r])), off = nm == -INFINITY ? 0.f : nm;
+                    const float a = exp2f(m[r] - off), e0 = exp2f(ls[0][r] - off), e1 = exp2f(ls[1][r] - off);
+                    acc[r].x = acc[r].x * a + v[0][r].x * e0 + v[1][r].x * e1;
+                    acc[r].y = acc[r].y * a + v[0][r].y * e0 + v[1][r].y * e1;
+                    acc[r].z = acc[r].z * a + v[0][r].z * e0 + v[1][r].z * e1;
+                    acc[r].w = acc[r].w * a + v[0][r].w * e0 + v[1][r].w * e1;
+                    sum[r] = sum[r] * a + e0 + e1;
+                    m[r] = nm;
+                }
+                if (!behind) break;
+                x[0] = __ffs(behind) - 1;
+                behind &= behind - 1;
+                fl[0] = first_piece[x[0]].flags;
+                n = 1;
+            }
+            const bool whole = (lead.flags & 2) && ends;    // all of it lies in this block
+            // row 0 of the block: of a (sequence, head) that comes from the block before it; row 1: of one that starts here
+            const int s = (lead.flags & 2) ? 1 : 0;
+            float *row = p.block_rows + ((int64_t)cta * 2 + s) * ROW;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (r >= heads) break;
+                const int head = quad * 4 + r;
+                const float f = !whole && sum[r] == 0.f ? 0.f : 1.f / sum[r];
+                if (whole) {
+                    if (lane * 4 < D)
+                        store4<T>((T *)p.o + ((int64_t)lead.b * p.num_q_heads + hq0 + head) * D + lane * 4, acc[r].x * f, acc[r].y * f,
+                                  acc[r].z * f, acc[r].w * f);
+                } else {
+                    if (lane * 4 < D)
+                        __stcg(reinterpret_cast<float4 *>(row + head * D + lane * 4),
+                               make_float4(acc[r].x * f, acc[r].y * f, acc[r].z * f, acc[r].w * f));
+                    if (lane == 0) __stcg(row + HC * D + head, log2f(sum[r]) + (m[r] == -INFINITY ? 0.f : m[r]));
+                }
+            }
+            if (!whole && quad == 0 && lane == 0) {
+                cross_f[s] = blocks.owner(lead.p0);
+                cross_n[s] = blocks.owner(lead.p0 + lead.nt - 1) - cross_f[s] + 1;
+                cross_b[s] = lead.b;
+                cross_hp[s] = lead.hp;
+                cross_valid[s] = 1;
             }
         }
     }
+    if (!all_leaders) return;       // (the same for every thread of the block)
     __threadfence();
     __syncthreads();
     if (tid < 2 && cross_valid[tid]) {
@@ -871,6 +927,12 @@ static bool fast_shape(const PoolViewQ8 &pv) {
     const int bs = pv.block_size;
     return (pv.head_dim == 64 || pv.head_dim == 128) && bs >= kHalf && (bs & (bs - 1)) == 0 &&
            pv.tile_bytes * pv.num_layers * pv.num_kv_heads < (1ll << 32) && pv.total_blocks < (1ll << 31);
+}
+// Positions of a launch whose sequences fill the table's rows stay below 2^30 (they are counted in 32 bits).
+static bool fast_positions(const PoolViewQ8 &pv, int batch, int group, int64_t cols) {
+    const int64_t tokens = std::min<int64_t>(cols * pv.block_size, 0x7fffffff);
+    const double per = (double)(ceil_div64(tokens, kTile) + kUnitCost) * pv.num_kv_heads * ((group + 3) / 4);
+    return per * batch < (double)(1 << 30);
 }
 // 16-byte loads of q and of the pool, 8-byte stores of o.
 static bool fast_aligned(const PoolViewQ8 &pv, const void *q, int64_t q_stride, const void *o) {
@@ -949,7 +1011,8 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
     int *flags = workspace && workspace_bytes >= kErrorBytes ? (int *)workspace : nullptr;
     const float scale_log2 = softmax_scale * kLog2e;
     const int group = num_q_heads / pv.num_kv_heads;
-    if (dtype != MKV_F32 && fast_shape(pv) && fast_aligned(pv, q, q_stride, o)) {
+    if (dtype != MKV_F32 && fast_shape(pv) && fast_aligned(pv, q, q_stride, o) &&
+        fast_positions(pv, batch, group, table_stride)) {
         int sms = 0;
         if ((st = mkv_sm_count(device, &sms))) return st;
         if (!workspace || workspace_bytes < mkv_attn_q8_workspace_bytes(device, batch, num_q_heads, pv.num_kv_heads, pv.head_dim))
@@ -974,7 +1037,7 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
         while ((kHalf << p.half_shift) < pv.block_size) ++p.half_shift;
         p.max_len = (int)std::min<int64_t>(table_stride * pv.block_size, 0x7fffffff);
         p.scale_log2 = scale_log2;
-        const int most = sms * kBlocksPerSm;
+        const int most = sms * kBlocksPerSm;    // (fast_positions keeps (most + 1) * step below 2^31)
         const int64_t positions = (int64_t)batch * (ceil_div64(max_seq_len, kTile) + kUnitCost) * pv.num_kv_heads * p.groups;
         const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, positions / (heads == 16 ? kWarpsWide : kWarps)));
         p.error_flags = (int *)workspace;
