@@ -495,7 +495,6 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         if (more && nb == -2) look_ahead();     // early, so that the next sequence's ids are there when it comes
         const uint4 scales = lds16(st + META), ma = lds16(st + META + 16);
         const int flags = (int)(ma.x & 0xffu);
-        const int tokens[2] = {(int)((ma.x >> 8) & 0xffu), (int)(ma.x >> 16)};
         busy = !(flags & 4);
 
         if (flags & 1) {    // first tile of a piece
@@ -558,99 +557,90 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
             }
         }
 
-        // ---- S^T = K Q^T
-        float sc[2][NT][4];
-#pragma unroll
+        // One half after the other in one body: unrolled, the two would overlap, but the code a block has to fetch before its
+        // first result would be twice as long.
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-            float part[NT][2][4];   // two chains, for the latency
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    part[n][0][e] = CODE == MKV_Q8_INT8 ? kinit[n][e & 1] : 0.f;
-                    part[n][1][e] = 0.f;
-                }
-#pragma unroll
-            for (int i = 0; i < KW / 4; ++i) {
-                const uint32_t at = st + h * HB + (k_at ^ (i << 4));
-                const uint4 x = lds16(at), y = lds16(at + HB / 2);      // tokens g and g + 8
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t a0, a1, a2, a3;
-                    widen_k<CODE>(xs[j], a0, a2);
-                    widen_k<CODE>(ys[j], a1, a3);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma(part[n][j & 1], a0, a1, a2, a3, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[h][n][e] = part[n][0][e] + part[n][1][e];
-        }
-        // ---- softmax: token g (elements 0, 1) and g + 8 (2, 3) of each half, heads 2t, 2t + 1
-        // The block's V scale joins the exponent: weights are 2^(score + log2 s_v - base), so that O accumulates across
-        // blocks as the tensor core leaves it, and the denominator takes them back over s_v.  A scale below 2^-100 (an
-        // all-zero block's, above all) counts as 2^-100, and does not move the maximum.
-        float iv[2];
-        bool above = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+            const uint32_t at = st + h * HB;
+            const int tokens = (int)((ma.x >> (8 + 8 * h)) & 0xffu);
             const float ks = __uint_as_float(h ? scales.y : scales.x), vs = __uint_as_float(h ? scales.w : scales.z);
+            // ---- S^T = K Q^T
+            float sc[NT][4];
+            {
+                float part[NT][2][4];   // two chains, for the latency
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        part[n][0][e] = CODE == MKV_Q8_INT8 ? kinit[n][e & 1] : 0.f;
+                        part[n][1][e] = 0.f;
+                    }
+#pragma unroll
+                for (int i = 0; i < KW / 4; ++i) {
+                    const uint4 x = lds16(at + (k_at ^ (i << 4))), y = lds16(at + (k_at ^ (i << 4)) + HB / 2);  // tokens g and g + 8
+                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t a0, a1, a2, a3;
+                        widen_k<CODE>(xs[j], a0, a2);
+                        widen_k<CODE>(ys[j], a1, a3);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma(part[n][j & 1], a0, a1, a2, a3, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[n][e] = part[n][0][e] + part[n][1][e];
+            }
+            // ---- softmax: token g (elements 0, 1) and g + 8 (2, 3), heads 2t, 2t + 1
+            // The block's V scale joins the exponent: weights are 2^(score + log2 s_v - base), so that O accumulates across
+            // blocks as the tensor core leaves it, and the denominator takes them back over s_v.  A scale below 2^-100 (an
+            // all-zero block's, above all) counts as 2^-100, and does not move the maximum.
             const float sv = vs < kLeastScale ? kLeastScale : vs;
-            float lv;
+            float lv, iv;
             asm("lg2.approx.f32 %0, %1;\n" : "=f"(lv) : "f"(sv));
-            asm("rcp.approx.f32 %0, %1;\n" : "=f"(iv[h]) : "f"(sv));
-            const bool on0 = g < tokens[h], on1 = g + 8 < tokens[h];
+            asm("rcp.approx.f32 %0, %1;\n" : "=f"(iv) : "f"(sv));
+            const bool on0 = g < tokens, on1 = g + 8 < tokens;
+            bool above = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float f0 = (kScaledQ ? qfac[n][0] : p.scale_log2) * ks, f1 = (kScaledQ ? qfac[n][1] : p.scale_log2) * ks;
-                sc[h][n][0] = on0 ? fmaf(sc[h][n][0], f0, lv) : -INFINITY;
-                sc[h][n][1] = on0 ? fmaf(sc[h][n][1], f1, lv) : -INFINITY;
-                sc[h][n][2] = on1 ? fmaf(sc[h][n][2], f0, lv) : -INFINITY;
-                sc[h][n][3] = on1 ? fmaf(sc[h][n][3], f1, lv) : -INFINITY;
+                sc[n][0] = on0 ? fmaf(sc[n][0], f0, lv) : -INFINITY;
+                sc[n][1] = on0 ? fmaf(sc[n][1], f1, lv) : -INFINITY;
+                sc[n][2] = on1 ? fmaf(sc[n][2], f0, lv) : -INFINITY;
+                sc[n][3] = on1 ? fmaf(sc[n][3], f1, lv) : -INFINITY;
+                above |= fmaxf(sc[n][0], sc[n][2]) > thr[n][0] || fmaxf(sc[n][1], sc[n][3]) > thr[n][1];
             }
-        }
-        float mx[NT][2];
+            if (__any_sync(0xffffffffu, above)) {   // the maxima settle after the first tiles of a piece
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                mx[n][e] = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
-                above |= mx[n][e] > thr[n][e];
-            }
-        if (__any_sync(0xffffffffu, above)) {   // the maxima settle after the first tiles of a piece
+                    for (int e = 0; e < 2; ++e) {
+                        float m = fmaxf(sc[n][e], sc[n][e + 2]);
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                        m = fmaxf(m, thr[n][e] - kLag);
+                        const float to = m == -INFINITY ? 0.f : m - kBoost;
+                        const float a = thr[n][e] == -INFINITY ? 1.f : ex2(base[n][e] - to);   // before: all weights were 0
+                        thr[n][e] = m + kLag;
+                        base[n][e] = to;
+                        l[n][e] *= a;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float m = mx[n][e];
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    m = fmaxf(m, thr[n][e] - kLag);
-                    const float to = m == -INFINITY ? 0.f : m - kBoost;
-                    const float a = thr[n][e] == -INFINITY ? 1.f : ex2(base[n][e] - to);   // before: all weights were 0
-                    thr[n][e] = m + kLag;
-                    base[n][e] = to;
-                    l[n][e] *= a;
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        o[n][i][e] *= a;
-                        o[n][i][e + 2] *= a;
+                        for (int i = 0; i < MT; ++i) {
+                            o[n][i][e] *= a;
+                            o[n][i][e + 2] *= a;
+                        }
                     }
-                }
-        }
-        uint32_t pb[2][NT][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
+            }
+            uint32_t pb[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float w0 = ex2(sc[h][n][0] - base[n][0]), w1 = ex2(sc[h][n][1] - base[n][1]);
-                const float w2 = ex2(sc[h][n][2] - base[n][0]), w3 = ex2(sc[h][n][3] - base[n][1]);
-                l[n][0] = fmaf(w0 + w2, iv[h], l[n][0]);
-                l[n][1] = fmaf(w1 + w3, iv[h], l[n][1]);
+                const float w0 = ex2(sc[n][0] - base[n][0]), w1 = ex2(sc[n][1] - base[n][1]);
+                const float w2 = ex2(sc[n][2] - base[n][0]), w3 = ex2(sc[n][3] - base[n][1]);
+                l[n][0] = fmaf(w0 + w2, iv, l[n][0]);
+                l[n][1] = fmaf(w1 + w3, iv, l[n][1]);
                 __half2 x = __floats2half2_rn(w0, w1), y = __floats2half2_rn(w2, w3);
                 if (DUP) {  // columns 4-7: what the rounding of columns 0-3 left over
                     const float2 fx = __half22float2(x), fy = __half22float2(y);
@@ -658,19 +648,18 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     x = t >= 2 ? rx : x;
                     y = t >= 2 ? ry : y;
                 }
-                pb[h][n][0] = transpose8x8(half2_bits(x));
-                pb[h][n][1] = transpose8x8(half2_bits(y));
+                pb[n][0] = transpose8x8(half2_bits(x));
+                pb[n][1] = transpose8x8(half2_bits(y));
             }
-        // ---- O^T += V^T P^T: row tile c has dim 16 c + 2 g in its row g and dim 16 c + 2 g + 1 in its row g + 8
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+            // ---- O^T += V^T P^T: row tile c has dim 16 c + 2 g in its row g and dim 16 c + 2 g + 1 in its row g + 8
+            // Behind the sequence's end any byte may stand, an e4m3 NaN among them, and 0 x NaN is NaN.
+            const bool cut = CODE == MKV_Q8_E4M3 && tokens < kHalf;
 #pragma unroll
             for (int c = 0; c < MT; c += 2) {
                 uint32_t w[4];      // (16-dim piece c: tokens 0-7, 8-15; piece c + 1: the same)
-                ldsm4_trans(w, st + h * HB + (v_at ^ (c << 4)));
-                if (CODE == MKV_Q8_E4M3 && tokens[h] < kHalf) {
-                    // behind the sequence's end any byte may stand, NaN among them, and 0 x NaN is NaN
-                    const int n = tokens[h] - 2 * t;
+                ldsm4_trans(w, at + (v_at ^ (c << 4)));
+                if (cut) {
+                    const int n = tokens - 2 * t;
                     const uint32_t lo = n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u, hi = n >= 10 ? 0xffffffffu : n == 9 ? 0xffffu : 0u;
                     w[0] &= lo; w[1] &= hi; w[2] &= lo; w[3] &= hi;
                 }
@@ -680,7 +669,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     widen_v<CODE>(w[2 * d], a0, a1);
                     widen_v<CODE>(w[2 * d + 1], a2, a3);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma(o[n][c + d], a0, a1, a2, a3, pb[h][n][0], pb[h][n][1]);
+                    for (int n = 0; n < NT; ++n) mma(o[n][c + d], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                 }
             }
         }
