@@ -198,21 +198,23 @@ __device__ __forceinline__ void store4(T *dst, float a, float b, float c, float 
     *reinterpret_cast<Four *>(dst) = v;
 }
 
-struct AttnQ8Params {
-    PoolViewQ8 pool;
-    const void *q;
-    void *o;
-    int64_t q_stride;
-    const int32_t *block_table;
+struct AttnQ8Params {       // what every launch reads stands together in front: constant memory is cold at a launch's start
+    const int32_t *seq_ids, *seq_lens, *block_table;
     int64_t table_cols;
-    int num_rows;
-    const int32_t *seq_ids, *seq_lens;
-    int batch, num_q_heads, group, groups;  // groups: units of up to HC query heads for each kv head
+    int batch, num_rows, max_len;           // max_len: tokens that a row of the table can hold
+    int num_q_heads, num_kv_heads, group, groups;  // groups: units of up to HC query heads for each kv head
     int cur_layer, half_shift;              // halves (16 tokens) of a block: 1 << half_shift
-    int max_len;                            // tokens that a row of the table can hold
+    int num_segments;
+    uint32_t total_blocks, tile_bytes, block_tiles;  // block_tiles: layers * kv heads
     float scale_log2;
-    int *error_flags, *arrive;
+    const uint8_t *k0, *v0;                 // segment 0
+    const float *ks0, *vs0;
+    const void *q;
+    int64_t q_stride;
+    void *o;
     float *head_rows, *block_rows;          // [worker] and [2 * block] rows of HC * D values + HC log-sums
+    int *error_flags, *arrive;
+    PoolViewQ8 pool;                        // (the elastic segments)
 };
 
 struct Piece {      // a (sequence, head) that a warp has some tiles of
@@ -247,11 +249,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Piece first_piece[WARPS], last_piece[WARPS];
     __shared__ int scan_w[WARPS];
-    __shared__ int4 start_at[WARPS];    // where a warp's range starts: batch index, its first position, length, table row
+    __shared__ int seq_from[WARPS * 32], seq_len[WARPS * 32], seq_row[WARPS * 32];
     __shared__ int cross_valid[2], cross_f[2], cross_n[2], cross_b[2], cross_hp[2], cross_last[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int P = p.pool.num_kv_heads * p.groups;
+    const int P = p.num_kv_heads * p.groups;
     uint8_t *ring_ptr = smem + warp * (STAGES * STAGE);
     const uint32_t ring = smem_addr(ring_ptr);
 
@@ -280,37 +282,22 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     if (lane == 0) first_piece[warp].flags = last_piece[warp].flags = 0;
     if (tid < 2) cross_valid[tid] = cross_last[tid] = 0;
     __syncthreads();
-    int total = 0, from = incl - mine;
+    int total = 0, before = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) from += scan_w[w];
+        if (w < warp) before += scan_w[w];
         total += scan_w[w];
     }
+    seq_from[tid] = before + incl - mine;
+    seq_len[tid] = my_len;
+    seq_row[tid] = my_row;
+    __syncthreads();
     // A position at least for each warp of a block, so that a piece that enters a block is its first warp's.
     const Shares blocks(total, max(min((int)gridDim.x, total / WARPS), 1));
     const int cta = blockIdx.x;
     if (total == 0 || cta >= blocks.n) return;
     const int lo = blocks.start(cta), hi = blocks.start(cta + 1);
     const Shares warps(hi - lo, WARPS);
-    if (mine > 0 && from < hi && from + mine > lo) {
-#pragma unroll 1
-        for (int w = 0; w < WARPS; ++w) {
-            const int x = lo + warps.start(w);
-            if (x < from || x >= from + mine) continue;
-            int b = tid * per, at = from, len = my_len, row = my_row;
-            if (per > 1) {
-                for (;; ++b) {      // (one of them holds x)
-                    len = __ldg(p.seq_lens + b);
-                    const int nt = tiles_of(len), c = nt > 0 ? (nt + kUnitCost) * P : 0;
-                    if (x < at + c || b + 1 == min((tid + 1) * per, p.batch)) break;
-                    at += c;
-                }
-                row = __ldg(p.seq_ids + b);
-            }
-            start_at[w] = make_int4(b, at, len, row);
-        }
-    }
-    __syncthreads();
     const int wlo = lo + warps.start(warp), whi = lo + warps.start(warp + 1);
 
     // ---- where the warp reads next: the same in every lane, the id windows apart -----------------------------------
@@ -320,7 +307,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     bool bad = false, more = false;
     int cb = 0, chp = 0, ch = 0, chg = 0, cnt = 0, cj = 0, cjend = 0, clen = 0, crow = 0, cbase = 0, crem = 0;
     int first_flag = 1;
-    int64_t uoff = 0;               // bytes of the unit's (layer, head) inside a block's codes
+    uint64_t uoff = 0;              // bytes of the unit's (layer, head) inside a block's codes
     int2 ids, ids_next;             // lane l: block ids of tile cbase + l's halves, and of the 32 tiles behind those
     int2 ids0_next = make_int2(-1, -1);  // ... of the first 32 tiles of the next sequence (nb; its row and length)
     int nb = -2, nrow = 0, nlen = 0;    // -1: there is none, -2: not looked for yet
@@ -355,7 +342,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         clen = min(clen, p.max_len);
     };
     auto enter_head = [&]() {
-        uoff = (int64_t)(p.cur_layer * p.pool.num_kv_heads + ch) * p.pool.tile_bytes;
+        uoff = (uint64_t)(uint32_t)(p.cur_layer * p.num_kv_heads + ch) * p.tile_bytes;
         cjend = min(cnt, crem);
         more = cj < cjend;
         cbase = cj;
@@ -363,12 +350,27 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         if (more) ids_next = load_ids(crow, cj + 32, cnt);
     };
     if (wlo < whi) {
-        const int4 at = start_at[warp];
-        cb = at.x;
-        clen = at.z;
-        crow = at.w;
+        // the last thread whose first position is not behind wlo holds it (one without positions shares its successor's)
+        int seg = 0;
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w)
+            if (seq_from[w * 32] <= wlo) seg = w;
+        const int i = seg * 32 + 31 - __clz(__ballot_sync(0xffffffffu, seq_from[seg * 32 + lane] <= wlo));
+        int at = seq_from[i];
+        cb = i * per;
+        clen = seq_len[i];
+        crow = seq_row[i];
+        if (per > 1) {      // ... in one of its sequences
+            for (;; ++cb) {
+                clen = __ldg(p.seq_lens + cb);
+                const int nt = tiles_of(clen), c = nt > 0 ? (nt + kUnitCost) * P : 0;
+                if (wlo < at + c || cb + 1 >= min((i + 1) * per, p.batch)) break;
+                at += c;
+            }
+            crow = __ldg(p.seq_ids + cb);
+        }
         enter_sequence();
-        const unsigned w = cnt + kUnitCost, rem = wlo - at.y;
+        const unsigned w = cnt + kUnitCost, rem = wlo - at;
         chp = min((int)(rem / w), P - 1);
         const int inside = (int)(rem - chp * w);
         cj = max(inside - kUnitCost, 0);
@@ -379,22 +381,26 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         enter_head();
     }
     const uint64_t lane16 = (uint64_t)lane * 16;
-    const uint32_t block_tiles = (uint32_t)(p.pool.num_layers * p.pool.num_kv_heads);
-    const uint32_t block_bytes = (uint32_t)p.pool.tile_bytes * block_tiles;
+    const uint32_t block_bytes = p.tile_bytes * p.block_tiles;
     // 16-byte piece i * 32 + lane of a half.  D = 128: piece c of token r goes to c ^ (r & 7); D = 64: two tokens share a
     // 128-byte line, whose pieces go to c ^ (line & 3).  Either way the reads below meet no conflict.
     const uint32_t put = (uint32_t)((lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
     auto issue_half = [&](uint32_t st, int h, uint32_t blk, int &tokens) {
-        if (tokens > 0 && blk < (uint64_t)p.pool.total_blocks) {
-            int seg = 0;
+        if (tokens > 0 && blk < p.total_blocks) {
             uint32_t row = blk;
-            if (p.pool.num_segments > 1) {
+            const uint8_t *k0 = p.k0, *v0 = p.v0;
+            const float *s0 = lane ? p.vs0 : p.ks0;
+            if (p.num_segments > 1) {
+                int seg;
                 int64_t r;
                 locate_block(p.pool, blk, seg, r);
                 row = (uint32_t)r;
+                k0 = p.pool.k_base[seg];
+                v0 = p.pool.v_base[seg];
+                s0 = lane ? p.pool.v_scale[seg] : p.pool.k_scale[seg];
             }
             const uint64_t off = (uint64_t)row * block_bytes + uoff + (uint32_t)(((2 * cj + h) & half_mask) * HB) + lane16;
-            const uint8_t *kt = p.pool.k_base[seg] + off, *vt = p.pool.v_base[seg] + off;
+            const uint8_t *kt = k0 + off, *vt = v0 + off;
 #pragma unroll
             for (int i = 0; i < HB / 512; ++i) {
                 const uint32_t to = st + h * HB + i * 512 + (D == 128 && (i & 1) ? put ^ 64 : put);
@@ -402,8 +408,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 cp16(to + 2 * HB, vt + i * 512);
             }
             if (lane < 2)
-                cp4(st + META + (lane * 2 + h) * 4, (lane ? p.pool.v_scale[seg] : p.pool.k_scale[seg]) +
-                                                        ((uint64_t)row * block_tiles + p.cur_layer * p.pool.num_kv_heads + ch));
+                cp4(st + META + (lane * 2 + h) * 4, s0 + ((uint64_t)row * p.block_tiles + (uint32_t)(p.cur_layer * p.num_kv_heads + ch)));
         } else {
             bad |= tokens > 0;
             tokens = 0;
@@ -1009,6 +1014,15 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
         const int heads = unit_heads(group);
         AttnQ8Params p;
         p.pool = pv;
+        p.num_kv_heads = pv.num_kv_heads;
+        p.num_segments = pv.num_segments;
+        p.total_blocks = (uint32_t)pv.total_blocks;
+        p.tile_bytes = (uint32_t)pv.tile_bytes;
+        p.block_tiles = (uint32_t)(pv.num_layers * pv.num_kv_heads);
+        p.k0 = pv.k_base[0];
+        p.v0 = pv.v_base[0];
+        p.ks0 = pv.k_scale[0];
+        p.vs0 = pv.v_scale[0];
         p.q = q;
         p.o = o;
         p.q_stride = q_stride;
