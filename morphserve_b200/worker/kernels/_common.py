@@ -24,6 +24,11 @@ def device_and_stream(t: torch.Tensor):
     return dev, torch.cuda.current_stream(dev).cuda_stream
 
 
+def raw_stream(dev: int) -> int:
+    """The handle of the current stream of device `dev`."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def make_pool(k_cache, v_cache, k_cache_new, v_cache_new, num_blocks_org, chunk_blocks) -> MkvPool:
     """Segment table for the C ABI: segment 0 = the original pool, segment 1+j =
     elastic chunk j (server/memory_utils.py:389-390 appends them in this order).
@@ -130,20 +135,22 @@ def workspace_q8(dev: int, stream: int, batch: int, hq: int, hkv: int, d: int):
             raise RuntimeError("mkv_attn_q8_workspace_bytes failed")
         _q8_bytes_cache[key] = need
     nbytes, zero = need
-    if dev == torch.cuda.current_device():
-        capturing = torch.cuda.is_current_stream_capturing()
+    # (captures of another device than the current one are noticed too: the current stream is then asked for there)
+    if dev == torch._C._cuda_getDevice():
+        capturing = torch._C._cuda_isCurrentStreamCapturing()
     else:
         with torch.cuda.device(dev):
-            capturing = torch.cuda.is_current_stream_capturing()
+            capturing = torch._C._cuda_isCurrentStreamCapturing()
     ws = None if capturing else _workspaces_q8.get((dev, stream))
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
-        ws[:zero].zero_()
+    if ws is None or ws[1] < nbytes:
+        t = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+        t[:zero].zero_()
+        ws = (t, nbytes)
         if not capturing:
             if len(_workspaces_q8) >= _MAX_WORKSPACES and (dev, stream) not in _workspaces_q8:
                 _workspaces_q8.pop(next(iter(_workspaces_q8)))
             _workspaces_q8[(dev, stream)] = ws
-    return ws, ws.numel()
+    return ws
 
 
 def read_attn_error_flags(dev: int) -> int:
@@ -151,7 +158,7 @@ def read_attn_error_flags(dev: int) -> int:
     entry pointed outside the pool.  (The 8-bit pool's launches inside captured graphs have words of their own, which
     are not among them.)"""
     out = 0
-    for (d, _), ws in list(_workspaces_q8.items()):
+    for (d, _), (ws, _) in list(_workspaces_q8.items()):
         if d == dev:
             out |= int(ws[:4].view(torch.int32).item())
     for (d, _), ws in list(_workspaces.items()):

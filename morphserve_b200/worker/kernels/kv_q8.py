@@ -18,12 +18,12 @@ brings its own scratch, so graphs share none.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 
 import torch
 
 from ..._lib import MKV_MAX_SEGMENTS, MkvPoolQ8, check, lib
-from ._common import device_and_stream, require_cuda, workspace_q8
+from ._common import raw_stream, require_cuda, workspace_q8
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}       # mkv_dtype
 _CODES = {torch.int8: 1, torch.float8_e4m3fn: 2}                        # mkv_q8_code
@@ -38,21 +38,31 @@ def alloc_kvcache_q8(num_blocks: int, model_config, engine_config, dtype: torch.
     return (*codes, *[torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)])
 
 
-def _segment(pool, i, k, v, ks, vs, dtype, device):
-    assert k.dtype == v.dtype == dtype and ks.dtype == vs.dtype == torch.float32
-    assert k.shape == v.shape and ks.shape == vs.shape and k.shape[:3] == ks.shape
+# mkv_pool_q8, packed rather than assigned field by field: the header, then one pointer of each kind a segment.
+_HEADER = struct.Struct("6i2q")
+_POINTER = struct.Struct("Q")
+_FIELDS = (MkvPoolQ8.k_base.offset, MkvPoolQ8.v_base.offset, MkvPoolQ8.k_scale.offset, MkvPoolQ8.v_scale.offset)
+
+
+def _segment(buf, i, k, v, ks, vs, dtype, shape, dev):
+    assert k.shape == shape and v.shape == shape and ks.shape == shape[:3] and vs.shape == shape[:3]
+    assert k.dtype is dtype and v.dtype is dtype and ks.dtype is torch.float32 and vs.dtype is torch.float32
     assert k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
-    assert k.device == device and v.device == device and ks.device == device and vs.device == device
-    pool.k_base[i] = k.data_ptr()
-    pool.v_base[i] = v.data_ptr()
-    pool.k_scale[i] = ks.data_ptr()
-    pool.v_scale[i] = vs.data_ptr()
+    assert k.get_device() == dev and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev
+    at = 8 * i
+    _POINTER.pack_into(buf, _FIELDS[0] + at, k.data_ptr())
+    _POINTER.pack_into(buf, _FIELDS[1] + at, v.data_ptr())
+    _POINTER.pack_into(buf, _FIELDS[2] + at, ks.data_ptr())
+    _POINTER.pack_into(buf, _FIELDS[3] + at, vs.data_ptr())
 
 
 def _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new, model_config,
-          engine_config, num_blocks_org, chunk_blocks) -> MkvPoolQ8:
-    require_cuda(k_cache, "k_cache")
-    dtype = k_cache.dtype
+          engine_config, num_blocks_org, chunk_blocks):
+    """(descriptor, shape of the original pool, device index)"""
+    dev = k_cache.get_device()
+    if dev < 0:
+        require_cuda(k_cache, "k_cache")
+    dtype, shape = k_cache.dtype, k_cache.shape
     code = _CODES.get(dtype)
     if code is None:
         raise RuntimeError(f"unsupported 8-bit KV dtype {dtype}")
@@ -60,40 +70,42 @@ def _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_
     if n_new + 1 > MKV_MAX_SEGMENTS:
         raise RuntimeError(f"too many elastic KV chunks ({n_new}); the library supports {MKV_MAX_SEGMENTS - 1}")
     assert len(v_cache_new) == n_new and len(k_scale_new) == n_new and len(v_scale_new) == n_new
-    blocks, layers, heads, bs, d = k_cache.shape
+    blocks, layers, heads, bs, d = shape
     assert heads == model_config.num_kv_heads and d == model_config.head_dim and bs == engine_config.block_size
-    pool = MkvPoolQ8()
-    pool.num_segments = 1 + n_new
-    pool.code = code
-    pool.num_layers = layers
-    pool.num_kv_heads = heads
-    pool.block_size = bs
-    pool.head_dim = d
-    pool.num_blocks_org = blocks
-    _segment(pool, 0, k_cache, v_cache, k_scale, v_scale, dtype, k_cache.device)
+    buf = MkvPoolQ8()
+    _segment(buf, 0, k_cache, v_cache, k_scale, v_scale, dtype, shape, dev)
     if n_new:
         if int(num_blocks_org) != blocks:
             raise RuntimeError("num_blocks_org is not the number of blocks of the original pool")
-        pool.chunk_blocks = int(chunk_blocks)
+        chunk_blocks = int(chunk_blocks)
+        chunk = torch.Size((chunk_blocks, layers, heads, bs, d))
         for j in range(n_new):
-            if tuple(k_cache_new[j].shape) != (pool.chunk_blocks, layers, heads, bs, d):
+            if k_cache_new[j].shape != chunk:
                 raise RuntimeError("elastic KV chunks must all hold kv_cache_new_block_size blocks of the pool's shape")
-            _segment(pool, 1 + j, k_cache_new[j], v_cache_new[j], k_scale_new[j], v_scale_new[j], dtype, k_cache.device)
-    return pool
+            _segment(buf, 1 + j, k_cache_new[j], v_cache_new[j], k_scale_new[j], v_scale_new[j], dtype, chunk, dev)
+    _HEADER.pack_into(buf, 0, 1 + n_new, code, layers, heads, bs, d, blocks, chunk_blocks if n_new else 0)
+    return buf, shape, dev
 
 
-def _rows(x, heads, d, device, name):
+def _rows(x, heads, d, dev):
     """Distance of two tokens, in elements, of rows [tokens, heads, head_dim] whose elements and heads are contiguous."""
-    assert x.dim() == 3 and x.shape[1] == heads and x.shape[2] == d, f"{name} is [tokens, {heads}, {d}]"
-    assert x.device == device, f"{name} is on another device than the cache"
-    assert (x.stride(2) == 1 or d == 1) and (x.stride(1) == d or heads == 1), f"{name}: elements and heads are contiguous"
-    return x.stride(0) if x.shape[0] > 1 else heads * d
+    shape, stride = x.shape, x.stride()
+    assert len(shape) == 3 and shape[1] == heads and shape[2] == d, f"rows are [tokens, {heads}, {d}]"
+    assert x.get_device() == dev, "rows are on another device than the cache"
+    assert (stride[2] == 1 or d == 1) and (stride[1] == d or heads == 1), "elements and heads of a row are contiguous"
+    return stride[0] if shape[0] > 1 else heads * d
 
 
-def _ints(device, **tensors):
-    for name, t in tensors.items():
-        assert t.dtype == torch.int32 and t.is_contiguous() and t.device == device, \
-            f"{name}: contiguous int32 on the cache's device"
+def _ints(x, dev, n, name):
+    assert x.dtype is torch.int32 and x.is_contiguous() and x.get_device() == dev and x.shape[0] >= n, \
+        f"{name}: contiguous int32 on the cache's device, one for each sequence"
+    return x.data_ptr()
+
+
+def _table(x, dev):
+    assert x.dtype is torch.int32 and x.is_contiguous() and x.get_device() == dev, "block_table: contiguous int32 on the cache's device"
+    rows, cols = x.shape
+    return x.data_ptr(), cols, rows
 
 
 def _dtype(x):
@@ -128,36 +140,30 @@ def store_kvcache_q8(
     block's scale and the token's holds, and where that is the token's the older codes are rounded again.  A sequence
     given more than once in one of the two parts: its last entry counts.  Sequences of length 0, ids outside the table
     and blocks outside the pool are skipped."""
-    pool = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new, model_config,
-                 engine_config, infer_state.num_blocks_org, infer_state.kv_cache_new_block_size)
-    device = k_cache.device
-    heads, d = pool.num_kv_heads, pool.head_dim
-    assert k.dtype == v.dtype and k.shape[0] == v.shape[0]
+    pool, shape, dev = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new,
+                             model_config, engine_config, infer_state.num_blocks_org, infer_state.kv_cache_new_block_size)
+    heads, d = shape[2], shape[4]
+    assert k.dtype is v.dtype and k.shape[0] == v.shape[0]
     dtype = _dtype(k)
-    ks, vs = _rows(k, heads, d, device, "k"), _rows(v, heads, d, device, "v")
-    seq_ids = infer_state.seq_ids
-    _ints(device, block_table=block_table, seq_ids=seq_ids)
+    ks, vs = _rows(k, heads, d, dev), _rows(v, heads, d, dev)
     n_pre, n_dec = infer_state.num_prefill_seqs, infer_state.num_decoding_seqs
     n_tok = infer_state.num_prefill_tokens if n_pre > 0 else 0
-    assert seq_ids.shape[0] >= n_pre + n_dec and k.shape[0] >= n_tok + n_dec
-    dev, stream = device_and_stream(k_cache)
+    assert k.shape[0] >= n_tok + n_dec
+    table, cols, rows = _table(block_table, dev)
+    seq_ids = _ints(infer_state.seq_ids, dev, n_pre + n_dec, "seq_ids")
+    stream = raw_stream(dev)
     if n_pre > 0:
-        starts, lens = infer_state.prefill_seq_start_locs, infer_state.prefill_seq_lens
-        _ints(device, prefill_seq_start_locs=starts, prefill_seq_lens=lens)
-        assert starts.shape[0] >= n_pre and lens.shape[0] >= n_pre
-        check(lib.mkv_store_kv_q8_prefill(
-            dev, stream, k.data_ptr(), v.data_ptr(), ks, vs, dtype, n_tok, pool, block_table.data_ptr(),
-            block_table.shape[1], block_table.shape[0], seq_ids.data_ptr(), starts.data_ptr(), lens.data_ptr(), n_pre,
-            int(infer_state.max_prefill_len), cur_layer), "mkv_store_kv_q8_prefill")
+        status = lib.mkv_store_kv_q8_prefill(
+            dev, stream, k.data_ptr(), v.data_ptr(), ks, vs, dtype, n_tok, pool, table, cols, rows, seq_ids,
+            _ints(infer_state.prefill_seq_start_locs, dev, n_pre, "prefill_seq_start_locs"),
+            _ints(infer_state.prefill_seq_lens, dev, n_pre, "prefill_seq_lens"), n_pre, int(infer_state.max_prefill_len), cur_layer)
+        check(status, "mkv_store_kv_q8_prefill")
     if n_dec > 0:
-        lens = infer_state.decoding_seq_lens
-        _ints(device, decoding_seq_lens=lens)
-        assert lens.shape[0] >= n_dec
         skip = n_tok * k.element_size()
-        check(lib.mkv_store_kv_q8_decode(
-            dev, stream, k.data_ptr() + skip * ks, v.data_ptr() + skip * vs, ks, vs, dtype, pool, block_table.data_ptr(),
-            block_table.shape[1], block_table.shape[0], seq_ids.data_ptr() + 4 * n_pre, lens.data_ptr(), n_dec,
-            cur_layer), "mkv_store_kv_q8_decode")
+        status = lib.mkv_store_kv_q8_decode(
+            dev, stream, k.data_ptr() + skip * ks, v.data_ptr() + skip * vs, ks, vs, dtype, pool, table, cols, rows,
+            seq_ids + 4 * n_pre, _ints(infer_state.decoding_seq_lens, dev, n_dec, "decoding_seq_lens"), n_dec, cur_layer)
+        check(status, "mkv_store_kv_q8_decode")
 
 
 def load_kvcache_q8(
@@ -185,21 +191,18 @@ def load_kvcache_q8(
     ``start_locs[i] + t - begins[i]`` of ``k`` and ``v`` - a cached prefix for a prefill attention that wants contiguous
     rows, or a sequence on its way into another pool.  Rows that no range reaches, and rows of tokens whose page is not
     in the table or the pool, are left as they were."""
-    pool = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new, model_config,
-                 engine_config, k_cache.shape[0], k_cache_new[0].shape[0] if len(k_cache_new) else 0)
-    device = k_cache.device
-    heads, d = pool.num_kv_heads, pool.head_dim
-    assert k.dtype == v.dtype and k.shape[0] == v.shape[0]
+    pool, shape, dev = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new,
+                             model_config, engine_config, k_cache.shape[0], k_cache_new[0].shape[0] if len(k_cache_new) else 0)
+    heads, d = shape[2], shape[4]
+    assert k.dtype is v.dtype and k.shape[0] == v.shape[0]
     dtype = _dtype(k)
-    ks, vs = _rows(k, heads, d, device, "k"), _rows(v, heads, d, device, "v")
+    ks, vs = _rows(k, heads, d, dev), _rows(v, heads, d, dev)
     n = seq_ids.shape[0]
-    _ints(device, block_table=block_table, seq_ids=seq_ids, begins=begins, ends=ends, start_locs=start_locs)
-    assert begins.shape[0] == n and ends.shape[0] == n and start_locs.shape[0] == n
-    dev, stream = device_and_stream(k_cache)
+    table, cols, rows = _table(block_table, dev)
     check(lib.mkv_load_kv_q8(
-        dev, stream, k.data_ptr(), v.data_ptr(), ks, vs, dtype, k.shape[0], pool, block_table.data_ptr(),
-        block_table.shape[1], block_table.shape[0], seq_ids.data_ptr(), begins.data_ptr(), ends.data_ptr(),
-        start_locs.data_ptr(), n, int(max_len), cur_layer), "mkv_load_kv_q8")
+        dev, raw_stream(dev), k.data_ptr(), v.data_ptr(), ks, vs, dtype, k.shape[0], pool, table, cols, rows,
+        _ints(seq_ids, dev, n, "seq_ids"), _ints(begins, dev, n, "begins"), _ints(ends, dev, n, "ends"),
+        _ints(start_locs, dev, n, "start_locs"), n, int(max_len), cur_layer), "mkv_load_kv_q8")
 
 
 def paged_attention_q8(
@@ -229,22 +232,20 @@ def paged_attention_q8(
     batch = infer_state.num_decoding_seqs
     if batch == 0:
         return
-    pool = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new, model_config,
-                 engine_config, infer_state.num_blocks_org, infer_state.kv_cache_new_block_size)
-    device = k_cache.device
-    hq, hkv, d = model_config.num_q_heads, pool.num_kv_heads, pool.head_dim
+    pool, shape, dev = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new,
+                             model_config, engine_config, infer_state.num_blocks_org, infer_state.kv_cache_new_block_size)
+    hq, hkv, bs, d = model_config.num_q_heads, shape[2], shape[3], shape[4]
     dtype = _dtype(q)
-    q_stride = _rows(q, hq, d, device, "q")
+    q_stride = _rows(q, hq, d, dev)
     assert q.shape[0] >= batch
-    assert o.dtype == q.dtype and o.is_contiguous() and o.device == device and o.numel() >= batch * hq * d
-    seq_ids, lens = infer_state.seq_ids, infer_state.decoding_seq_lens
+    assert o.dtype is q.dtype and o.is_contiguous() and o.get_device() == dev and o.numel() >= batch * hq * d
     n_pre = infer_state.num_prefill_seqs
-    _ints(device, block_table=block_table, seq_ids=seq_ids, decoding_seq_lens=lens)
-    assert seq_ids.shape[0] >= n_pre + batch and lens.shape[0] >= batch
-    max_len = getattr(infer_state, "max_decoding_len", None) or engine_config.max_blocks_per_seq * pool.block_size
-    dev, stream = device_and_stream(k_cache)
+    table, cols, rows = _table(block_table, dev)
+    seq_ids = _ints(infer_state.seq_ids, dev, n_pre + batch, "seq_ids") + 4 * n_pre
+    lens = _ints(infer_state.decoding_seq_lens, dev, batch, "decoding_seq_lens")
+    max_len = infer_state.max_decoding_len or engine_config.max_blocks_per_seq * bs
+    stream = raw_stream(dev)
     ws, ws_bytes = workspace_q8(dev, stream, batch, hq, hkv, d)
     check(lib.mkv_paged_attention_q8(
-        dev, stream, q.data_ptr(), q_stride, o.data_ptr(), dtype, pool, block_table.data_ptr(), block_table.shape[1],
-        block_table.shape[0], seq_ids.data_ptr() + 4 * n_pre, lens.data_ptr(), batch, hq, cur_layer,
-        float(infer_state.softmax_scale), int(max_len), ws.data_ptr(), ws_bytes), "mkv_paged_attention_q8")
+        dev, stream, q.data_ptr(), q_stride, o.data_ptr(), dtype, pool, table, cols, rows, seq_ids, lens, batch, hq,
+        cur_layer, infer_state.softmax_scale, max_len, ws.data_ptr(), ws_bytes), "mkv_paged_attention_q8")

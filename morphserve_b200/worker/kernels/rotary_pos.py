@@ -13,7 +13,7 @@ import math
 import torch
 
 from ..._lib import check, lib
-from ._common import device_and_stream, require_cuda
+from ._common import raw_stream, require_cuda
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}       # mkv_dtype
 
@@ -78,6 +78,18 @@ def rotary_inv_freq(model_config, device="cuda"):
     return inv.to(device), float(attention_scale)
 
 
+_INTS = {torch.int32: 4, torch.int64: 8}
+_Strides = C.c_int64 * 8
+
+
+def _strides(x, n, heads, d):
+    """Distances of two tokens and of two heads; elements are contiguous, nothing overlaps."""
+    s = x.stride()
+    assert s[2] == 1, "elements are contiguous"
+    assert (n <= 1 or s[0] >= d) and (heads <= 1 or s[1] >= d), "tokens and heads do not overlap"
+    return s
+
+
 def rotary_embedding_positions(
     q: torch.Tensor,                # [num_tokens, num_q_heads, head_dim]
     k: torch.Tensor,                # [num_tokens, num_kv_heads, head_dim]
@@ -94,27 +106,34 @@ def rotary_embedding_positions(
     not overlap q and k).  fp16, bf16 or fp32, computed in fp32 and rounded once.  Elements are contiguous; tokens and
     heads may lie any distance apart, so q and k may be views of one fused projection.  Any position that a 64-bit float
     holds keeps its angle to about 2^-24 of half a turn."""
-    require_cuda(q, "q")
-    q_out = q if q_out is None else q_out
-    k_out = k if k_out is None else k_out
-    device, n = q.device, q.shape[0]
-    for t in (q, k, q_out, k_out):
-        assert t.dim() == 3 and t.shape[0] == n and t.dtype == q.dtype and t.device == device
-        assert t.stride(2) == 1 and t.shape[2] == q.shape[2], "elements are contiguous, one head_dim"
-        assert t.shape[0] <= 1 or t.stride(0) >= t.shape[2], "tokens do not overlap"
-        assert t.shape[1] <= 1 or t.stride(1) >= t.shape[2], "heads do not overlap"
-    assert q_out.shape == q.shape and k_out.shape == k.shape
-    code = _DTYPES.get(q.dtype)
+    dev = q.get_device()
+    if dev < 0:
+        require_cuda(q, "q")
+    shape, k_shape, dtype = q.shape, k.shape, q.dtype
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise RuntimeError(f"unsupported dtype {q.dtype}")
-    assert positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous() and positions.shape == (n,)
-    assert inv_freq.dtype == torch.float64 and inv_freq.is_contiguous() and inv_freq.dim() == 1
-    assert positions.device == device and inv_freq.device == device
-    assert 2 * inv_freq.shape[0] <= q.shape[2], "inv_freq has at most head_dim / 2 entries"
-    dev, stream = device_and_stream(q)
-    strides = (C.c_int64 * 8)(q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                              q_out.stride(0), q_out.stride(1), k_out.stride(0), k_out.stride(1))
+        raise RuntimeError(f"unsupported dtype {dtype}")
+    n, hq, d = shape
+    hkv = k_shape[1]
+    assert len(k_shape) == 3 and k_shape[0] == n and k_shape[2] == d and k.dtype is dtype and k.get_device() == dev
+    qs, ks = _strides(q, n, hq, d), _strides(k, n, hkv, d)
+    qos, kos = qs, ks
+    if q_out is None:
+        q_out = q
+    else:
+        assert q_out.shape == shape and q_out.dtype is dtype and q_out.get_device() == dev
+        qos = _strides(q_out, n, hq, d)
+    if k_out is None:
+        k_out = k
+    else:
+        assert k_out.shape == k_shape and k_out.dtype is dtype and k_out.get_device() == dev
+        kos = _strides(k_out, n, hkv, d)
+    assert positions.dtype in _INTS and positions.is_contiguous() and positions.shape == shape[:1]
+    assert inv_freq.dtype is torch.float64 and inv_freq.is_contiguous() and inv_freq.dim() == 1
+    assert positions.get_device() == dev and inv_freq.get_device() == dev
+    pairs = inv_freq.shape[0]
+    assert 2 * pairs <= d, "inv_freq has at most head_dim / 2 entries"
     check(lib.mkv_rotary_positions(
-        dev, stream, q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), strides, positions.data_ptr(),
-        positions.element_size(), inv_freq.data_ptr(), inv_freq.shape[0], bool(interleaved), attention_scale, n,
-        q.shape[1], k.shape[1], q.shape[2], code), "mkv_rotary_positions")
+        dev, raw_stream(dev), q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+        _Strides(qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1]), positions.data_ptr(), _INTS[positions.dtype],
+        inv_freq.data_ptr(), pairs, bool(interleaved), attention_scale, n, hq, hkv, d, code), "mkv_rotary_positions")

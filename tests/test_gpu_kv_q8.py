@@ -363,7 +363,7 @@ def test_attention_leaves_out_pages_that_are_not_there(mk, d):
     c.check_attention(o, qn, lens=lens, ids=ids)
     assert torch.isnan(o[2]).all() and torch.isnan(o[3]).all()
     assert read_attn_error_flags(0) & 1
-    for ws in _workspaces_q8.values():
+    for ws, _ in _workspaces_q8.values():
         ws[:4].zero_()
 
 
