@@ -3,6 +3,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_q8.cuh"
 
@@ -51,225 +52,300 @@ __device__ __forceinline__ int64_t page_of(const PoolViewQ8 &p, const int32_t *t
     return tile_index(p, r, layer, 0);
 }
 
-// V elements of T at once: as few and as wide loads as the alignment allows.
+// ------------------------------------------------------------------ access
+// A thread's piece of a row: V elements of T, V codes.  V = 16: 32 bytes of a 16-bit type in one access (64 of fp32 in two), 16
+// bytes of codes.  V = 1 for rows that are not so aligned.
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Pack {
-    T x[V];
-};
-
-template <typename T, int V>
-__device__ __forceinline__ void load_pack(const T *src, float (&x)[V]) {
-    const Pack<T, V> p = *reinterpret_cast<const Pack<T, V> *>(src);
+struct Piece {
+    static constexpr int WORDS = V * (int)sizeof(T) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T *src) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = value_of<T>(p.x[i]);
-}
-
-// Largest absolute value, as the bits of an fp32 number: the integer order puts infinity and NaN on top.
-template <int V>
-__device__ __forceinline__ uint32_t peak_bits(const float (&x)[V], uint32_t peak) {
+        for (int i = 0; i < WORDS; i += 8)
+            asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]),
+                           "=r"(w[i + 7])
+                         : "l"(reinterpret_cast<const uint32_t *>(src) + i));
+    }
+    __device__ __forceinline__ void store(T *dst) const {
 #pragma unroll
-    for (int i = 0; i < V; ++i) peak = max(peak, __float_as_uint(x[i]) & 0x7fffffffu);
-    return peak;
-}
-
-template <int CODE, int V>
-__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&x)[V], float inv) {
-    if constexpr (V % 4 == 0) {
-        Pack<uint32_t, V / 4> p;
+        for (int i = 0; i < WORDS; i += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(reinterpret_cast<uint32_t *>(dst) + i), "r"(w[i]),
+                         "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                         : "memory");
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = *reinterpret_cast<const __half2 *>(&w[i >> 1]);
+            return (i & 1) ? __high2float(h) : __low2float(h);
+        } else
+            return __uint_as_float((i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    }
+    __device__ __forceinline__ void set2(int i, float a, float b) {     // elements i, i + 1
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __float_as_uint(a);
+            w[i + 1] = __float_as_uint(b);
+        } else {
+            struct alignas(4) Two { T x, y; } t{rounded<T>(a), rounded<T>(b)};
+            w[i >> 1] = *reinterpret_cast<const uint32_t *>(&t);
+        }
+    }
+    // Largest absolute value, as the bits of an fp32 number: the integer order puts infinity and NaN on top.
+    __device__ __forceinline__ uint32_t peak(uint32_t most) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) most = max(most, __float_as_uint(get(i)) & 0x7fffffffu);
+        return most;
+    }
+    template <int CODE>
+    __device__ __forceinline__ void store_codes(uint8_t *dst, float inv) const {
+        uint32_t c[V / 4];
 #pragma unroll
         for (int i = 0; i < V / 4; ++i)
-            p.x[i] = inv > 0.f ? encode4<CODE>(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], inv) : 0u;
-        *reinterpret_cast<Pack<uint32_t, V / 4> *>(dst) = p;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) dst[i] = inv > 0.f ? encode1<CODE>(x[i], inv) : (uint8_t)0;
+            c[i] = inv > 0.f ? encode4<CODE>(get(4 * i), get(4 * i + 1), get(4 * i + 2), get(4 * i + 3), inv) : 0u;
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(c[0], c[1], c[2], c[3]);
     }
+};
+template <typename T>
+struct Piece<T, 1> {
+    T x;
+    __device__ __forceinline__ void load(const T *src) { x = *src; }
+    __device__ __forceinline__ uint32_t peak(uint32_t most) const { return max(most, __float_as_uint(value_of<T>(x)) & 0x7fffffffu); }
+    template <int CODE>
+    __device__ __forceinline__ void store_codes(uint8_t *dst, float inv) const {
+        *dst = inv > 0.f ? encode1<CODE>(value_of<T>(x), inv) : (uint8_t)0;
+    }
+};
+
+struct StoreQ8Args {
+    const void *k, *v;
+    int64_t k_stride, v_stride, num_tokens;
+    const int32_t *block_table;
+    int64_t table_cols;
+    const int32_t *seq_ids, *start_locs, *seq_lens;
+    int num_rows, num_seqs, cur_layer;
+    PoolViewQ8 pool;
+};
+
+// Threads of a block: one warp for each (head, K or V) of a page, up to 16; blockIdx.z takes the next 16.
+constexpr int kItemWarps = 16;
+
+// Whether a later entry with tokens names the same sequence: then that one counts.  (All threads of the block.)
+__device__ __forceinline__ bool named_again(const StoreQ8Args &a, int i, int row) {
+    bool again = false;
+    for (int j = i + 1 + threadIdx.x; j < a.num_seqs; j += blockDim.x) again |= a.seq_ids[j] == row && a.seq_lens[j] > 0;
+    return __syncthreads_or(again);
 }
 
 // ------------------------------------------------------------------ prefill scatter
-// One warp per (block, head, K or V): the block's peak, then its codes.  grid = (logical blocks, prompts).
-template <typename T, int CODE, int V>
-__global__ void store_q8_prefill_kernel(const T *__restrict__ k, const T *__restrict__ v, int64_t k_stride, int64_t v_stride,
-                                        int64_t num_tokens, const __grid_constant__ PoolViewQ8 pool,
-                                        const int32_t *__restrict__ block_table, int64_t table_stride, int num_rows,
-                                        const int32_t *__restrict__ seq_ids, const int32_t *__restrict__ start_locs,
-                                        const int32_t *__restrict__ seq_lens, int num_seqs, int cur_layer) {
+// grid = (logical blocks, prompts, heads / 8).  A warp takes one (page, head, K or V): its rows go into registers with every load
+// in flight at once (NV pieces a thread; 4 KiB a warp at 16 x 128 fp16), the peak is a butterfly, the codes leave as one
+// contiguous tile.  NV = 0: pages that do not fit are read twice.
+template <typename T, int CODE, int V, int NV>
+__global__ void __launch_bounds__(kItemWarps * 32) store_q8_prefill_kernel(const __grid_constant__ StoreQ8Args a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int D = pool.head_dim, bs = pool.block_size, Hkv = pool.num_kv_heads;
-    for (int i = blockIdx.y; i < num_seqs; i += gridDim.y) {
-        const int row = seq_ids[i];
-        const int64_t start = start_locs[i];
-        const int64_t len = min((int64_t)seq_lens[i], start < 0 ? 0 : num_tokens - start);
+    const int D = a.pool.head_dim, bs = a.pool.block_size, Hkv = a.pool.num_kv_heads, vecs = D / V;
+    const int item0 = blockIdx.z * warps + warp;
+    for (int i = blockIdx.y; i < a.num_seqs; i += gridDim.y) {
+        const int row = a.seq_ids[i];
+        const int64_t start = a.start_locs[i];
+        const int64_t len = min((int64_t)a.seq_lens[i], start < 0 ? 0 : a.num_tokens - start);
         if ((int64_t)blockIdx.x * bs >= len) continue;
-        bool again = false;  // the same sequence further on: that one counts
-        for (int j = i + 1 + lane; j < num_seqs; j += 32) again |= seq_ids[j] == row && seq_lens[j] > 0;
-        if (__any_sync(0xffffffffu, again)) continue;
+        if (named_again(a, i, row)) continue;
         for (int64_t lb = blockIdx.x; lb * bs < len; lb += gridDim.x) {
             int seg = 0;
-            const int64_t tile0 = page_of(pool, block_table, table_stride, num_rows, row, (int)min(lb, table_stride), cur_layer, seg);
+            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, (int)min(lb, a.table_cols), a.cur_layer, seg);
             if (tile0 < 0) continue;
-            const int ntok = (int)min((int64_t)bs, len - lb * bs);
-            const int vecs = D / V, total = ntok * vecs;
-            for (int item = warp; item < 2 * Hkv; item += warps) {
+            const int total = (int)min((int64_t)bs, len - lb * bs) * vecs;
+            for (int item = item0; item < 2 * Hkv; item += gridDim.z * warps) {
                 const int h = item >> 1, which = item & 1;
-                const T *src = (which ? v : k) + (start + lb * bs) * (which ? v_stride : k_stride) + (int64_t)h * D;
-                const int64_t stride = which ? v_stride : k_stride;
+                const int64_t stride = which ? a.v_stride : a.k_stride;
+                const T *src = (const T *)(which ? a.v : a.k) + (start + lb * bs) * stride + (int64_t)h * D;
+                uint8_t *dst = (which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + (tile0 + h) * a.pool.tile_bytes;
                 uint32_t peak = 0;
-                for (int e = lane; e < total; e += 32) {
-                    float x[V];
-                    load_pack<T, V>(src + (e / vecs) * stride + (e % vecs) * V, x);
-                    peak = peak_bits<V>(x, peak);
+                float s;
+                if constexpr (NV > 0) {
+                    Piece<T, V> x[NV];
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) {
+                        const int e = lane + 32 * j;
+                        if (e < total) x[j].load(src + (e / vecs) * stride + (e % vecs) * V);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (lane + 32 * j < total) peak = x[j].peak(peak);
+                    s = scale_of<CODE>(__reduce_max_sync(0xffffffffu, peak));
+                    const float inv = inverse_of(s);
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (lane + 32 * j < total) x[j].template store_codes<CODE>(dst + (lane + 32 * j) * V, inv);
+                } else {
+                    Piece<T, V> x;
+                    for (int e = lane; e < total; e += 32) {
+                        x.load(src + (e / vecs) * stride + (e % vecs) * V);
+                        peak = x.peak(peak);
+                    }
+                    s = scale_of<CODE>(__reduce_max_sync(0xffffffffu, peak));
+                    const float inv = inverse_of(s);
+                    for (int e = lane; e < total; e += 32) {
+                        x.load(src + (e / vecs) * stride + (e % vecs) * V);
+                        x.template store_codes<CODE>(dst + (int64_t)e * V, inv);
+                    }
                 }
-                peak = __reduce_max_sync(0xffffffffu, peak);
-                const float s = scale_of<CODE>(peak), inv = inverse_of(s);
-                uint8_t *dst = (which ? pool.v_base[seg] : pool.k_base[seg]) + (tile0 + h) * pool.tile_bytes;
-                for (int e = lane; e < total; e += 32) {
-                    float x[V];
-                    load_pack<T, V>(src + (e / vecs) * stride + (e % vecs) * V, x);
-                    store_codes<CODE, V>(dst + (int64_t)e * V, x, inv);
-                }
-                if (lane == 0) (which ? pool.v_scale[seg] : pool.k_scale[seg])[tile0 + h] = s;
+                if (lane == 0) (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile0 + h] = s;
             }
         }
     }
 }
 
 // ------------------------------------------------------------------ decode append
-// One warp per (sequence, head, K or V): nobody else touches the tile in this launch.
+// grid = (sequences, heads / 8).  One warp for each (sequence, head, K or V): nobody else touches the tile in this launch.
 template <typename T, int CODE, int V>
-__global__ void store_q8_decode_kernel(const T *__restrict__ k, const T *__restrict__ v, int64_t k_stride, int64_t v_stride,
-                                       const __grid_constant__ PoolViewQ8 pool, const int32_t *__restrict__ block_table,
-                                       int64_t table_stride, int num_rows, const int32_t *__restrict__ seq_ids,
-                                       const int32_t *__restrict__ seq_lens, int batch, int cur_layer) {
-    const int lane = threadIdx.x & 31;
-    const int64_t wid = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const int D = pool.head_dim, bs = pool.block_size, Hkv = pool.num_kv_heads;
-    if (wid >= (int64_t)batch * Hkv * 2) return;
-    const int b = (int)(wid / (2 * Hkv)), item = (int)(wid - (int64_t)b * 2 * Hkv), h = item >> 1, which = item & 1;
-    const int len = seq_lens[b], row = seq_ids[b];
-    bool again = false;
-    for (int j = b + 1 + lane; j < batch; j += 32) again |= seq_ids[j] == row && seq_lens[j] > 0;
-    if (__any_sync(0xffffffffu, again) || len <= 0) return;
+__global__ void __launch_bounds__(kItemWarps * 32) store_q8_decode_kernel(const __grid_constant__ StoreQ8Args a) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int D = a.pool.head_dim, bs = a.pool.block_size, Hkv = a.pool.num_kv_heads;
+    const int b = blockIdx.x, len = a.seq_lens[b], row = a.seq_ids[b];
+    if (len <= 0) return;
     const int lb = (len - 1) / bs, slot = (len - 1) - lb * bs;
     int seg = 0;
-    const int64_t tile0 = page_of(pool, block_table, table_stride, num_rows, row, lb, cur_layer, seg);
-    if (tile0 < 0) return;
-    const T *src = (which ? v + b * v_stride : k + b * k_stride) + (int64_t)h * D;
-    float *scale = (which ? pool.v_scale[seg] : pool.k_scale[seg]) + tile0 + h;
-    uint8_t *tile = (which ? pool.v_base[seg] : pool.k_base[seg]) + (tile0 + h) * pool.tile_bytes;
-    const float held = *scale;
-    uint32_t peak = 0;
-    for (int e = lane; e < D / V; e += 32) {
-        float x[V];
-        load_pack<T, V>(src + e * V, x);
-        peak = peak_bits<V>(x, peak);
-    }
-    peak = __reduce_max_sync(0xffffffffu, peak);
-    const float fresh = scale_of<CODE>(peak);
-    const float s = slot == 0 ? fresh : larger_scale(held, fresh), inv = inverse_of(s);
-    for (int e = lane; e < D / V; e += 32) {
-        float x[V];
-        load_pack<T, V>(src + e * V, x);
-        store_codes<CODE, V>(tile + (int64_t)slot * D + e * V, x, inv);
-    }
-    if (slot > 0 && s > held) {  // the codes before it to the new scale
-        const float ratio = __fmul_rn(held, inv);
-        for (int e = lane; e < slot * D / V; e += 32) {
-            uint8_t *at = tile + (int64_t)e * V;
-            float x[V];
-            if constexpr (V % 4 == 0) {
-                const Pack<uint32_t, V / 4> p = *reinterpret_cast<const Pack<uint32_t, V / 4> *>(at);
+    const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, lb, a.cur_layer, seg);
+    if (named_again(a, b, row) || tile0 < 0) return;
+    for (int item = blockIdx.y * warps + warp; item < 2 * Hkv; item += gridDim.y * warps) {
+        const int h = item >> 1, which = item & 1;
+        const T *src = (const T *)(which ? a.v : a.k) + b * (which ? a.v_stride : a.k_stride) + (int64_t)h * D;
+        float *scale = (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg]) + tile0 + h;
+        uint8_t *tile = (which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + (tile0 + h) * a.pool.tile_bytes;
+        const float held = *scale;
+        uint32_t peak = 0;
+        Piece<T, V> x;
+        for (int e = lane; e < D / V; e += 32) {
+            x.load(src + e * V);
+            peak = x.peak(peak);
+        }
+        const float fresh = scale_of<CODE>(__reduce_max_sync(0xffffffffu, peak));
+        const float s = slot == 0 ? fresh : larger_scale(held, fresh), inv = inverse_of(s);
+        for (int e = lane; e < D / V; e += 32) {
+            if (D / V > 32) x.load(src + e * V);    // (a row that fits the warp is still there)
+            x.template store_codes<CODE>(tile + (int64_t)slot * D + e * V, inv);
+        }
+        if (slot > 0 && s > held) {  // the codes before it to the new scale
+            const float ratio = __fmul_rn(held, inv);
+            if constexpr (V == 16) {
+                constexpr int U = 4;    // 2 KiB of codes in flight: the other 15 slots of a 16 x 128 tile at once
+                const int total = slot * D / 16;
+                for (int e0 = lane; e0 < total; e0 += 32 * U) {
+                    uint4 c[U];
 #pragma unroll
-                for (int i = 0; i < V / 4; ++i) {
-                    const float4 f = decode4<CODE>(p.x[i]);
-                    x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
+                    for (int u = 0; u < U; ++u)
+                        if (e0 + 32 * u < total) c[u] = reinterpret_cast<const uint4 *>(tile)[e0 + 32 * u];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (e0 + 32 * u >= total) break;
+                        uint32_t w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 f = decode4<CODE>(w[i]);
+                            w[i] = ratio > 0.f ? encode4<CODE>(f.x, f.y, f.z, f.w, ratio) : 0u;
+                        }
+                        reinterpret_cast<uint4 *>(tile)[e0 + 32 * u] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 }
             } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) x[i] = decode1<CODE>(at[i]);
+                for (int e = lane; e < slot * D; e += 32) tile[e] = ratio > 0.f ? encode1<CODE>(decode1<CODE>(tile[e]), ratio) : (uint8_t)0;
             }
-            store_codes<CODE, V>(at, x, ratio);
         }
+        if (lane == 0) *scale = s;
     }
-    if (lane == 0) *scale = s;
 }
 
 // ------------------------------------------------------------------ gather
-// One warp per (block, head, K or V).  grid = (blocks of the longest range, ranges).
+struct LoadQ8Args {
+    void *k, *v;
+    int64_t k_stride, v_stride, num_out_rows;
+    const int32_t *block_table;
+    int64_t table_cols;
+    const int32_t *seq_ids, *begins, *ends, *start_locs;
+    int num_rows, num_seqs, cur_layer;
+    PoolViewQ8 pool;
+};
+
+// grid = (pages of the longest range, ranges, heads / 8).  One warp for each (page, head, K or V); U pieces of codes in flight.
 template <typename T, int CODE, int V>
-__global__ void load_q8_kernel(T *__restrict__ k, T *__restrict__ v, int64_t k_stride, int64_t v_stride, int64_t num_out_rows,
-                               const __grid_constant__ PoolViewQ8 pool, const int32_t *__restrict__ block_table,
-                               int64_t table_stride, int num_rows, const int32_t *__restrict__ seq_ids,
-                               const int32_t *__restrict__ begins, const int32_t *__restrict__ ends,
-                               const int32_t *__restrict__ start_locs, int num_seqs, int cur_layer) {
+__global__ void __launch_bounds__(kItemWarps * 32) load_q8_kernel(const __grid_constant__ LoadQ8Args a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int D = pool.head_dim, bs = pool.block_size, Hkv = pool.num_kv_heads, vecs = D / V;
-    for (int i = blockIdx.y; i < num_seqs; i += gridDim.y) {
-        const int row = seq_ids[i], begin = max(begins[i], 0);
-        const int64_t shift = (int64_t)start_locs[i] - begins[i];  // output row of token t: t + shift
-        const int64_t end = min((int64_t)ends[i], num_out_rows - shift);
+    const int D = a.pool.head_dim, bs = a.pool.block_size, Hkv = a.pool.num_kv_heads, vecs = D / V;
+    for (int i = blockIdx.y; i < a.num_seqs; i += gridDim.y) {
+        const int row = a.seq_ids[i], first_tok = a.begins[i], begin = max(first_tok, 0);
+        const int64_t shift = (int64_t)a.start_locs[i] - first_tok;  // output row of token t: t + shift
+        const int64_t end = min((int64_t)a.ends[i], a.num_out_rows - shift);
         for (int64_t lb = begin / bs + blockIdx.x; lb * bs < end; lb += gridDim.x) {
             int seg = 0;
-            const int64_t tile0 = page_of(pool, block_table, table_stride, num_rows, row, (int)min(lb, table_stride), cur_layer, seg);
+            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, (int)min(lb, a.table_cols), a.cur_layer, seg);
             if (tile0 < 0) continue;
             const int64_t t0 = max((int64_t)begin, lb * bs), t1 = min(end, (lb + 1) * bs);
             const int64_t first = max(t0, -shift);  // a negative start_locs entry reaches no row in front of the output
             const int total = (int)(t1 - first) * vecs;
-            for (int item = warp; item < 2 * Hkv; item += warps) {
+            for (int item = blockIdx.z * warps + warp; item < 2 * Hkv; item += gridDim.z * warps) {
                 const int h = item >> 1, which = item & 1;
-                const float s = (which ? pool.v_scale[seg] : pool.k_scale[seg])[tile0 + h];
-                const uint8_t *tile = (which ? pool.v_base[seg] : pool.k_base[seg]) + (tile0 + h) * pool.tile_bytes +
+                const int64_t stride = which ? a.v_stride : a.k_stride;
+                const float s = (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile0 + h];
+                const uint8_t *tile = (which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + (tile0 + h) * a.pool.tile_bytes +
                                       (first - lb * bs) * D;
-                const int64_t stride = which ? v_stride : k_stride;
-                T *dst = (which ? v : k) + (first + shift) * stride + (int64_t)h * D;
-                for (int e = lane; e < total; e += 32) {
-                    Pack<T, V> out;
-                    if constexpr (V % 4 == 0) {
-                        const Pack<uint32_t, V / 4> p = *reinterpret_cast<const Pack<uint32_t, V / 4> *>(tile + (int64_t)e * V);
+                T *dst = (T *)(which ? a.v : a.k) + (first + shift) * stride + (int64_t)h * D;
+                if constexpr (V == 16) {
+                    constexpr int U = 4;
+                    for (int e0 = lane; e0 < total; e0 += 32 * U) {
+                        uint4 c[U];
 #pragma unroll
-                        for (int j = 0; j < V / 4; ++j) {
-                            const float4 f = decode4<CODE>(p.x[j]);
-                            out.x[4 * j] = rounded<T>(f.x * s);
-                            out.x[4 * j + 1] = rounded<T>(f.y * s);
-                            out.x[4 * j + 2] = rounded<T>(f.z * s);
-                            out.x[4 * j + 3] = rounded<T>(f.w * s);
+                        for (int u = 0; u < U; ++u)
+                            if (e0 + 32 * u < total) c[u] = __ldg(reinterpret_cast<const uint4 *>(tile) + e0 + 32 * u);
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            const int e = e0 + 32 * u;
+                            if (e >= total) break;
+                            const uint32_t w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+                            Piece<T, V> out;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float4 f = decode4<CODE>(w[j]);
+                                out.set2(4 * j, f.x * s, f.y * s);
+                                out.set2(4 * j + 2, f.z * s, f.w * s);
+                            }
+                            out.store(dst + (e / vecs) * stride + (e % vecs) * V);
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) out.x[j] = rounded<T>(decode1<CODE>(tile[(int64_t)e * V + j]) * s);
                     }
-                    *reinterpret_cast<Pack<T, V> *>(dst + (e / vecs) * stride + (e % vecs) * V) = out;
+                } else {
+                    for (int e = lane; e < total; e += 32) dst[(e / vecs) * stride + e % vecs] = rounded<T>(decode1<CODE>(tile[e]) * s);
                 }
             }
         }
     }
 }
 
-// Elements per access: 16 bytes of the model's type where rows, strides and bases allow it, else one element.
-static bool wide_ok(const PoolViewQ8 &pv, const void *k, const void *v, int64_t k_stride, int64_t v_stride, int dtype, int *vec) {
-    const int w = 16 / dtype_bytes(dtype);
-    *vec = w;
-    if (pv.head_dim % w != 0 || k_stride % w != 0 || v_stride % w != 0) return false;
-    if ((((uintptr_t)k | (uintptr_t)v) & 15) != 0) return false;
+// Whether rows and pool allow 16 elements (32 bytes and more) and 16 codes at once.
+static bool wide_ok(const PoolViewQ8 &pv, const void *k, const void *v, int64_t k_stride, int64_t v_stride, int dtype) {
+    const int64_t size = dtype_bytes(dtype);
+    if (pv.head_dim % 16 != 0) return false;
+    if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * size) | (uintptr_t)(v_stride * size)) & 31) != 0) return false;
     for (int i = 0; i < pv.num_segments; ++i)
-        if ((((uintptr_t)pv.k_base[i] | (uintptr_t)pv.v_base[i]) & (w - 1)) != 0) return false;
+        if ((((uintptr_t)pv.k_base[i] | (uintptr_t)pv.v_base[i]) & 15) != 0) return false;
     return true;
 }
 
-// Calls f with (T{}, code tag, vector tag).
+// Calls f with (T{}, code tag, elements of a piece).
 template <int N> struct Int { static constexpr int value = N; };
 template <typename F>
 static void dispatch(int dtype, int code, bool wide, F &&f) {
-    auto with_code = [&](auto t, auto w) {
+    auto with_code = [&](auto t) {
         if (code == MKV_Q8_INT8) {
-            if (wide) f(t, Int<MKV_Q8_INT8>{}, w); else f(t, Int<MKV_Q8_INT8>{}, Int<1>{});
+            if (wide) f(t, Int<MKV_Q8_INT8>{}, Int<16>{}); else f(t, Int<MKV_Q8_INT8>{}, Int<1>{});
         } else {
-            if (wide) f(t, Int<MKV_Q8_E4M3>{}, w); else f(t, Int<MKV_Q8_E4M3>{}, Int<1>{});
+            if (wide) f(t, Int<MKV_Q8_E4M3>{}, Int<16>{}); else f(t, Int<MKV_Q8_E4M3>{}, Int<1>{});
         }
     };
-    if (dtype == MKV_F16) with_code(__half{}, Int<8>{});
-    else if (dtype == MKV_BF16) with_code(__nv_bfloat16{}, Int<8>{});
-    else with_code(float{}, Int<4>{});
+    if (dtype == MKV_F16) with_code(__half{});
+    else if (dtype == MKV_BF16) with_code(__nv_bfloat16{});
+    else with_code(float{});
 }
 
 static int check_rows(const PoolViewQ8 &pv, int64_t k_stride, int64_t v_stride, int dtype) {
@@ -277,6 +353,9 @@ static int check_rows(const PoolViewQ8 &pv, int64_t k_stride, int64_t v_stride, 
     const int64_t row = (int64_t)pv.num_kv_heads * pv.head_dim;
     return k_stride < row || v_stride < row ? MKV_ERR_SHAPE : MKV_OK;
 }
+
+static int item_warps(const PoolViewQ8 &pv) { return std::min(2 * pv.num_kv_heads, kItemWarps); }
+static unsigned item_blocks(const PoolViewQ8 &pv) { return (unsigned)std::min<int64_t>(ceil_div64(2 * pv.num_kv_heads, kItemWarps), 65535); }
 
 }  // namespace mkv
 
@@ -288,24 +367,31 @@ int mkv_store_kv_q8_prefill(int device, void *stream, const void *k, const void 
                             int dtype, int64_t num_tokens, const mkv_pool_q8 *pool, const int32_t *block_table,
                             int64_t table_stride, int num_rows, const int32_t *seq_ids, const int32_t *start_locs,
                             const int32_t *seq_lens, int num_seqs, int max_seq_len, int cur_layer) {
-    PoolViewQ8 pv;
-    int st = validate_pool_q8(pool, &pv);
+    StoreQ8Args a;
+    int st = validate_pool_q8(pool, &a.pool);
     if (st) return st;
     if (num_seqs < 0 || max_seq_len < 0 || table_stride < 1 || num_rows < 0 || num_tokens < 0) return MKV_ERR_SHAPE;
-    if ((st = check_rows(pv, k_stride, v_stride, dtype))) return st;
-    if (cur_layer < 0 || cur_layer >= pv.num_layers) return MKV_ERR_RANGE;
+    if ((st = check_rows(a.pool, k_stride, v_stride, dtype))) return st;
+    if (cur_layer < 0 || cur_layer >= a.pool.num_layers) return MKV_ERR_RANGE;
     if (num_seqs == 0 || max_seq_len == 0) return MKV_OK;
     if (!k || !v || !block_table || !seq_ids || !seq_lens || !start_locs) return MKV_ERR_NULL;
+    a.k = k; a.v = v; a.k_stride = k_stride; a.v_stride = v_stride; a.num_tokens = num_tokens;
+    a.block_table = block_table; a.table_cols = table_stride; a.num_rows = num_rows;
+    a.seq_ids = seq_ids; a.start_locs = start_locs; a.seq_lens = seq_lens; a.num_seqs = num_seqs; a.cur_layer = cur_layer;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return set_cuda_error(guard.err);
-    int vec;
-    const bool wide = wide_ok(pv, k, v, k_stride, v_stride, dtype, &vec);
-    const dim3 grid((unsigned)ceil_div64(max_seq_len, pv.block_size), (unsigned)std::min(num_seqs, 65535));
-    dispatch(dtype, pv.code, wide, [&](auto t, auto code, auto w) {
+    const dim3 grid((unsigned)ceil_div64(max_seq_len, a.pool.block_size), (unsigned)std::min(num_seqs, 65535), item_blocks(a.pool));
+    const int threads = item_warps(a.pool) * 32;
+    const int64_t pieces = a.pool.tile_bytes / 16;
+    dispatch(dtype, a.pool.code, wide_ok(a.pool, k, v, k_stride, v_stride, dtype), [&](auto t, auto code, auto w) {
         using T = decltype(t);
-        store_q8_prefill_kernel<T, decltype(code)::value, decltype(w)::value><<<grid, 256, 0, (cudaStream_t)stream>>>(
-            (const T *)k, (const T *)v, k_stride, v_stride, num_tokens, pv, block_table, table_stride, num_rows, seq_ids,
-            start_locs, seq_lens, num_seqs, cur_layer);
+        constexpr int CODE = decltype(code)::value, V = decltype(w)::value;
+        cudaStream_t s = (cudaStream_t)stream;
+        if constexpr (V == 16) {    // a tile of up to 4 KiB of 16-bit rows (8 KiB of fp32) stays in registers
+            if (pieces <= 64) return store_q8_prefill_kernel<T, CODE, V, 2><<<grid, threads, 0, s>>>(a);
+            if (pieces <= 128) return store_q8_prefill_kernel<T, CODE, V, 4><<<grid, threads, 0, s>>>(a);
+        }
+        store_q8_prefill_kernel<T, CODE, V, 0><<<grid, threads, 0, s>>>(a);
     });
     MKV_LAUNCH_CHECK();
     return MKV_OK;
@@ -314,25 +400,23 @@ int mkv_store_kv_q8_prefill(int device, void *stream, const void *k, const void 
 int mkv_store_kv_q8_decode(int device, void *stream, const void *k, const void *v, int64_t k_stride, int64_t v_stride,
                            int dtype, const mkv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
                            int num_rows, const int32_t *seq_ids, const int32_t *seq_lens, int batch, int cur_layer) {
-    PoolViewQ8 pv;
-    int st = validate_pool_q8(pool, &pv);
+    StoreQ8Args a;
+    int st = validate_pool_q8(pool, &a.pool);
     if (st) return st;
     if (batch < 0 || table_stride < 1 || num_rows < 0) return MKV_ERR_SHAPE;
-    if ((st = check_rows(pv, k_stride, v_stride, dtype))) return st;
-    if (cur_layer < 0 || cur_layer >= pv.num_layers) return MKV_ERR_RANGE;
+    if ((st = check_rows(a.pool, k_stride, v_stride, dtype))) return st;
+    if (cur_layer < 0 || cur_layer >= a.pool.num_layers) return MKV_ERR_RANGE;
     if (batch == 0) return MKV_OK;
     if (!k || !v || !block_table || !seq_ids || !seq_lens) return MKV_ERR_NULL;
-    const int64_t blocks = ceil_div64((int64_t)batch * pv.num_kv_heads * 2, 4);
-    if (blocks > 0x7fffffff) return MKV_ERR_SHAPE;
+    a.k = k; a.v = v; a.k_stride = k_stride; a.v_stride = v_stride; a.num_tokens = batch;
+    a.block_table = block_table; a.table_cols = table_stride; a.num_rows = num_rows;
+    a.seq_ids = seq_ids; a.start_locs = nullptr; a.seq_lens = seq_lens; a.num_seqs = batch; a.cur_layer = cur_layer;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return set_cuda_error(guard.err);
-    int vec;
-    const bool wide = wide_ok(pv, k, v, k_stride, v_stride, dtype, &vec);
-    dispatch(dtype, pv.code, wide, [&](auto t, auto code, auto w) {
-        using T = decltype(t);
-        store_q8_decode_kernel<T, decltype(code)::value, decltype(w)::value><<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(
-            (const T *)k, (const T *)v, k_stride, v_stride, pv, block_table, table_stride, num_rows, seq_ids, seq_lens, batch,
-            cur_layer);
+    const dim3 grid((unsigned)batch, item_blocks(a.pool));
+    dispatch(dtype, a.pool.code, wide_ok(a.pool, k, v, k_stride, v_stride, dtype), [&](auto t, auto code, auto w) {
+        store_q8_decode_kernel<decltype(t), decltype(code)::value, decltype(w)::value>
+            <<<grid, item_warps(a.pool) * 32, 0, (cudaStream_t)stream>>>(a);
     });
     MKV_LAUNCH_CHECK();
     return MKV_OK;
@@ -342,25 +426,25 @@ int mkv_load_kv_q8(int device, void *stream, void *k, void *v, int64_t k_stride,
                    int64_t num_out_rows, const mkv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
                    int num_rows, const int32_t *seq_ids, const int32_t *begins, const int32_t *ends,
                    const int32_t *start_locs, int num_seqs, int max_len, int cur_layer) {
-    PoolViewQ8 pv;
-    int st = validate_pool_q8(pool, &pv);
+    LoadQ8Args a;
+    int st = validate_pool_q8(pool, &a.pool);
     if (st) return st;
     if (num_seqs < 0 || max_len < 0 || table_stride < 1 || num_rows < 0 || num_out_rows < 0) return MKV_ERR_SHAPE;
-    if ((st = check_rows(pv, k_stride, v_stride, dtype))) return st;
-    if (cur_layer < 0 || cur_layer >= pv.num_layers) return MKV_ERR_RANGE;
+    if ((st = check_rows(a.pool, k_stride, v_stride, dtype))) return st;
+    if (cur_layer < 0 || cur_layer >= a.pool.num_layers) return MKV_ERR_RANGE;
     if (num_seqs == 0 || max_len == 0 || num_out_rows == 0) return MKV_OK;
     if (!k || !v || !block_table || !seq_ids || !begins || !ends || !start_locs) return MKV_ERR_NULL;
+    a.k = k; a.v = v; a.k_stride = k_stride; a.v_stride = v_stride; a.num_out_rows = num_out_rows;
+    a.block_table = block_table; a.table_cols = table_stride; a.num_rows = num_rows;
+    a.seq_ids = seq_ids; a.begins = begins; a.ends = ends; a.start_locs = start_locs;
+    a.num_seqs = num_seqs; a.cur_layer = cur_layer;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return set_cuda_error(guard.err);
-    int vec;
-    const bool wide = wide_ok(pv, k, v, k_stride, v_stride, dtype, &vec);
     // a range that starts inside a block touches one block more
-    const dim3 grid((unsigned)(ceil_div64(max_len, pv.block_size) + 1), (unsigned)std::min(num_seqs, 65535));
-    dispatch(dtype, pv.code, wide, [&](auto t, auto code, auto w) {
-        using T = decltype(t);
-        load_q8_kernel<T, decltype(code)::value, decltype(w)::value><<<grid, 256, 0, (cudaStream_t)stream>>>(
-            (T *)k, (T *)v, k_stride, v_stride, num_out_rows, pv, block_table, table_stride, num_rows, seq_ids, begins, ends,
-            start_locs, num_seqs, cur_layer);
+    const dim3 grid((unsigned)(ceil_div64(max_len, a.pool.block_size) + 1), (unsigned)std::min(num_seqs, 65535), item_blocks(a.pool));
+    dispatch(dtype, a.pool.code, wide_ok(a.pool, k, v, k_stride, v_stride, dtype), [&](auto t, auto code, auto w) {
+        load_q8_kernel<decltype(t), decltype(code)::value, decltype(w)::value>
+            <<<grid, item_warps(a.pool) * 32, 0, (cudaStream_t)stream>>>(a);
     });
     MKV_LAUNCH_CHECK();
     return MKV_OK;
