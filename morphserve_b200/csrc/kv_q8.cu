@@ -62,7 +62,7 @@ struct Piece {
     __device__ __forceinline__ void load(const T *src) {
 #pragma unroll
         for (int i = 0; i < WORDS; i += 8)
-            asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+            asm("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
                          : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]),
                            "=r"(w[i + 7])
                          : "l"(reinterpret_cast<const uint32_t *>(src) + i));
@@ -91,11 +91,19 @@ struct Piece {
             w[i >> 1] = *reinterpret_cast<const uint32_t *>(&t);
         }
     }
-    // Largest absolute value, as the bits of an fp32 number: the integer order puts infinity and NaN on top.
+    // Largest absolute value, as the type's own bits (16-bit types: two maxima side by side): the integer order puts
+    // infinity and NaN on top.  peak_bits() makes an fp32 number's bits of it.
     __device__ __forceinline__ uint32_t peak(uint32_t most) const {
 #pragma unroll
-        for (int i = 0; i < V; ++i) most = max(most, __float_as_uint(get(i)) & 0x7fffffffu);
+        for (int i = 0; i < WORDS; ++i)
+            most = sizeof(T) == 4 ? max(most, w[i] & 0x7fffffffu) : __vmaxu2(most, w[i] & 0x7fff7fffu);
         return most;
+    }
+    static __device__ __forceinline__ uint32_t peak_bits(uint32_t most) {
+        if constexpr (sizeof(T) == 4) return most;
+        const uint32_t m = max(most & 0xffffu, most >> 16);
+        if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+        return m << 16;
     }
     template <int CODE>
     __device__ __forceinline__ void store_codes(uint8_t *dst, float inv) const {
@@ -111,6 +119,7 @@ struct Piece<T, 1> {
     T x;
     __device__ __forceinline__ void load(const T *src) { x = *src; }
     __device__ __forceinline__ uint32_t peak(uint32_t most) const { return max(most, __float_as_uint(value_of<T>(x)) & 0x7fffffffu); }
+    static __device__ __forceinline__ uint32_t peak_bits(uint32_t most) { return most; }
     template <int CODE>
     __device__ __forceinline__ void store_codes(uint8_t *dst, float inv) const {
         *dst = inv > 0.f ? encode1<CODE>(value_of<T>(x), inv) : (uint8_t)0;
@@ -124,11 +133,14 @@ struct StoreQ8Args {
     int64_t table_cols;
     const int32_t *seq_ids, *start_locs, *seq_lens;
     int num_rows, num_seqs, cur_layer;
+    uint32_t vecs_magic;        // ceil(2^32 / pieces of a row)
     PoolViewQ8 pool;
 };
 
-// Threads of a block: one warp for each (head, K or V) of a page, up to 16; blockIdx.z takes the next 16.
-constexpr int kItemWarps = 16;
+// Threads of a block: one warp for each head of a page, up to 8 (the decode append: for each (head, K or V), up to 16);
+// the grid's last dimension takes the heads behind those.
+constexpr int kHeadWarps = 8, kItemWarps = 16;
+constexpr int kLoadThreads = 256, kLoadFlight = 4;
 
 // Whether a later entry with tokens names the same sequence: then that one counts.  (All threads of the block.)
 __device__ __forceinline__ bool named_again(const StoreQ8Args &a, int i, int row) {
@@ -138,61 +150,68 @@ __device__ __forceinline__ bool named_again(const StoreQ8Args &a, int i, int row
 }
 
 // ------------------------------------------------------------------ prefill scatter
-// grid = (logical blocks, prompts, heads / 8).  A warp takes one (page, head, K or V): its rows go into registers with every load
-// in flight at once (NV pieces a thread; 4 KiB a warp at 16 x 128 fp16), the peak is a butterfly, the codes leave as one
-// contiguous tile.  NV = 0: pages that do not fit are read twice.
+// grid = (pages of the longest prompt, prompts, heads / 8).  A warp takes one head of a page, K and then V: the rows go into registers with
+// every load in flight at once (NV pieces a thread; 4 KiB a warp at 16 x 128 fp16), the peak is a butterfly, the codes leave
+// as one contiguous tile.  NV = 0: pages that do not fit are read twice.
 template <typename T, int CODE, int V, int NV>
-__global__ void __launch_bounds__(kItemWarps * 32) store_q8_prefill_kernel(const __grid_constant__ StoreQ8Args a) {
+__device__ __forceinline__ float store_tile(const StoreQ8Args &a, const T *src, int stride, uint8_t *dst, int total, int vecs, int lane) {
+    uint32_t peak = 0;
+    if constexpr (NV > 0) {
+        Piece<T, V> x[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = min(lane + 32 * j, total - 1), tok = (int)__umulhi((uint32_t)e, a.vecs_magic);  // behind the end: the last one again
+            x[j].load(src + tok * stride + (e - tok * vecs) * V);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) peak = x[j].peak(peak);
+        const float s = scale_of<CODE>(__reduce_max_sync(0xffffffffu, Piece<T, V>::peak_bits(peak))), inv = inverse_of(s);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (lane + 32 * j < total) x[j].template store_codes<CODE>(dst + (lane + 32 * j) * V, inv);
+        return s;
+    } else {
+        Piece<T, V> x;
+        for (int e = lane; e < total; e += 32) {
+            x.load(src + (int64_t)(e / vecs) * stride + (e % vecs) * V);
+            peak = x.peak(peak);
+        }
+        const float s = scale_of<CODE>(__reduce_max_sync(0xffffffffu, Piece<T, V>::peak_bits(peak))), inv = inverse_of(s);
+        for (int e = lane; e < total; e += 32) {
+            x.load(src + (int64_t)(e / vecs) * stride + (e % vecs) * V);
+            x.template store_codes<CODE>(dst + (int64_t)e * V, inv);
+        }
+        return s;
+    }
+}
+
+template <typename T, int CODE, int V, int NV>
+__global__ void __launch_bounds__(kHeadWarps * 32, sizeof(T) == 4 ? 2 : 4) store_q8_prefill_kernel(const __grid_constant__ StoreQ8Args a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int D = a.pool.head_dim, bs = a.pool.block_size, Hkv = a.pool.num_kv_heads, vecs = D / V;
-    const int item0 = blockIdx.z * warps + warp;
     for (int i = blockIdx.y; i < a.num_seqs; i += gridDim.y) {
         const int row = a.seq_ids[i];
         const int64_t start = a.start_locs[i];
-        const int64_t len = min((int64_t)a.seq_lens[i], start < 0 ? 0 : a.num_tokens - start);
+        const int len = (int)min((int64_t)a.seq_lens[i], start < 0 ? 0 : a.num_tokens - start);
         if ((int64_t)blockIdx.x * bs >= len) continue;
-        if (named_again(a, i, row)) continue;
-        for (int64_t lb = blockIdx.x; lb * bs < len; lb += gridDim.x) {
+        bool again = false;
+        for (int lb = blockIdx.x; (int64_t)lb * bs < len; lb += gridDim.x) {
             int seg = 0;
-            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, (int)min(lb, a.table_cols), a.cur_layer, seg);
+            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, lb, a.cur_layer, seg);
+            if (lb == (int)blockIdx.x) again = named_again(a, i, row);
+            if (again) break;
             if (tile0 < 0) continue;
-            const int total = (int)min((int64_t)bs, len - lb * bs) * vecs;
-            for (int item = item0; item < 2 * Hkv; item += gridDim.z * warps) {
-                const int h = item >> 1, which = item & 1;
-                const int64_t stride = which ? a.v_stride : a.k_stride;
-                const T *src = (const T *)(which ? a.v : a.k) + (start + lb * bs) * stride + (int64_t)h * D;
-                uint8_t *dst = (which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + (tile0 + h) * a.pool.tile_bytes;
-                uint32_t peak = 0;
-                float s;
-                if constexpr (NV > 0) {
-                    Piece<T, V> x[NV];
-#pragma unroll
-                    for (int j = 0; j < NV; ++j) {
-                        const int e = lane + 32 * j;
-                        if (e < total) x[j].load(src + (e / vecs) * stride + (e % vecs) * V);
-                    }
-#pragma unroll
-                    for (int j = 0; j < NV; ++j)
-                        if (lane + 32 * j < total) peak = x[j].peak(peak);
-                    s = scale_of<CODE>(__reduce_max_sync(0xffffffffu, peak));
-                    const float inv = inverse_of(s);
-#pragma unroll
-                    for (int j = 0; j < NV; ++j)
-                        if (lane + 32 * j < total) x[j].template store_codes<CODE>(dst + (lane + 32 * j) * V, inv);
-                } else {
-                    Piece<T, V> x;
-                    for (int e = lane; e < total; e += 32) {
-                        x.load(src + (e / vecs) * stride + (e % vecs) * V);
-                        peak = x.peak(peak);
-                    }
-                    s = scale_of<CODE>(__reduce_max_sync(0xffffffffu, peak));
-                    const float inv = inverse_of(s);
-                    for (int e = lane; e < total; e += 32) {
-                        x.load(src + (e / vecs) * stride + (e % vecs) * V);
-                        x.template store_codes<CODE>(dst + (int64_t)e * V, inv);
-                    }
+            const int total = min(bs, len - lb * bs) * vecs;
+            for (int h = blockIdx.z * warps + warp; h < Hkv; h += gridDim.z * warps) {
+                const int64_t tile = tile0 + h;
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+                    const int64_t stride = which ? a.v_stride : a.k_stride;
+                    const T *src = (const T *)(which ? a.v : a.k) + (start + lb * bs) * stride + (int64_t)h * D;
+                    uint8_t *dst = (which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + tile * a.pool.tile_bytes;
+                    const float s = store_tile<T, CODE, V, NV>(a, src, (int)stride, dst, total, vecs, lane);
+                    if (lane == 0) (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile] = s;
                 }
-                if (lane == 0) (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile0 + h] = s;
             }
         }
     }
@@ -222,7 +241,7 @@ __global__ void __launch_bounds__(kItemWarps * 32) store_q8_decode_kernel(const 
             x.load(src + e * V);
             peak = x.peak(peak);
         }
-        const float fresh = scale_of<CODE>(__reduce_max_sync(0xffffffffu, peak));
+        const float fresh = scale_of<CODE>(__reduce_max_sync(0xffffffffu, Piece<T, V>::peak_bits(peak)));
         const float s = slot == 0 ? fresh : larger_scale(held, fresh), inv = inverse_of(s);
         for (int e = lane; e < D / V; e += 32) {
             if (D / V > 32) x.load(src + e * V);    // (a row that fits the warp is still there)
@@ -266,56 +285,67 @@ struct LoadQ8Args {
     int64_t table_cols;
     const int32_t *seq_ids, *begins, *ends, *start_locs;
     int num_rows, num_seqs, cur_layer;
+    uint32_t vecs_magic;        // ceil(2^32 / pieces of a row)
     PoolViewQ8 pool;
 };
 
-// grid = (pages of the longest range, ranges, heads / 8).  One warp for each (page, head, K or V); U pieces of codes in flight.
+// grid = (pages of the longest range, ranges, parts of a page).  A page is (head, K or V) tiles of `chunks` x 32 pieces (V codes
+// each); a warp takes kLoadFlight such chunks at a time, all of their loads before the first store.
 template <typename T, int CODE, int V>
-__global__ void __launch_bounds__(kItemWarps * 32) load_q8_kernel(const __grid_constant__ LoadQ8Args a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+__global__ void __launch_bounds__(kLoadThreads, 4) load_q8_kernel(const __grid_constant__ LoadQ8Args a) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = a.pool.head_dim, bs = a.pool.block_size, Hkv = a.pool.num_kv_heads, vecs = D / V;
     for (int i = blockIdx.y; i < a.num_seqs; i += gridDim.y) {
-        const int row = a.seq_ids[i], first_tok = a.begins[i], begin = max(first_tok, 0);
+        const int row = a.seq_ids[i], first_tok = a.begins[i];
         const int64_t shift = (int64_t)a.start_locs[i] - first_tok;  // output row of token t: t + shift
         const int64_t end = min((int64_t)a.ends[i], a.num_out_rows - shift);
-        for (int64_t lb = begin / bs + blockIdx.x; lb * bs < end; lb += gridDim.x) {
+        const int64_t begin = max((int64_t)max(first_tok, 0), -shift);   // (a negative start_locs entry reaches no row in front of the output)
+        if (begin >= end) continue;
+        for (int lb = (int)begin / bs + blockIdx.x; (int64_t)lb * bs < end; lb += gridDim.x) {
             int seg = 0;
-            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, (int)min(lb, a.table_cols), a.cur_layer, seg);
+            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, lb, a.cur_layer, seg);
             if (tile0 < 0) continue;
-            const int64_t t0 = max((int64_t)begin, lb * bs), t1 = min(end, (lb + 1) * bs);
-            const int64_t first = max(t0, -shift);  // a negative start_locs entry reaches no row in front of the output
-            const int total = (int)(t1 - first) * vecs;
-            for (int item = blockIdx.z * warps + warp; item < 2 * Hkv; item += gridDim.z * warps) {
-                const int h = item >> 1, which = item & 1;
-                const int64_t stride = which ? a.v_stride : a.k_stride;
-                const float s = (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile0 + h];
-                const uint8_t *tile = (which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + (tile0 + h) * a.pool.tile_bytes +
-                                      (first - lb * bs) * D;
-                T *dst = (T *)(which ? a.v : a.k) + (first + shift) * stride + (int64_t)h * D;
+            const int first = max((int)begin, lb * bs);
+            const int total = ((int)min(end, ((int64_t)lb + 1) * bs) - first) * vecs, chunks = (total + 31) / 32, all = chunks * 2 * Hkv;
+            const int tile_bytes = (int)a.pool.tile_bytes, skip = (int)(first - lb * bs) * D, step = gridDim.z * (kLoadThreads / 32);
+            for (int c0 = blockIdx.z * (kLoadThreads / 32) + warp; c0 < all; c0 += kLoadFlight * step) {
                 if constexpr (V == 16) {
-                    constexpr int U = 4;
-                    for (int e0 = lane; e0 < total; e0 += 32 * U) {
-                        uint4 c[U];
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-                            if (e0 + 32 * u < total) c[u] = __ldg(reinterpret_cast<const uint4 *>(tile) + e0 + 32 * u);
-#pragma unroll
-                        for (int u = 0; u < U; ++u) {
-                            const int e = e0 + 32 * u;
-                            if (e >= total) break;
-                            const uint32_t w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
-                            Piece<T, V> out;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float4 f = decode4<CODE>(w[j]);
-                                out.set2(4 * j, f.x * s, f.y * s);
-                                out.set2(4 * j + 2, f.z * s, f.w * s);
-                            }
-                            out.store(dst + (e / vecs) * stride + (e % vecs) * V);
+                    uint4 x[kLoadFlight];
+                    float s[kLoadFlight];
+                    T *dst[kLoadFlight];
+    #pragma unroll
+                    for (int u = 0; u < kLoadFlight; ++u) {     // (behind the last piece: that one again, and nothing is written)
+                        const int c = min(c0 + u * step, all - 1), item = c / chunks, e = (c - item * chunks) * 32 + lane, at = min(e, total - 1);
+                        const int h = item >> 1, which = item & 1, tok = (int)__umulhi((uint32_t)at, a.vecs_magic);
+                        const int64_t stride = which ? a.v_stride : a.k_stride, tile = tile0 + h;
+                        x[u] = __ldg(reinterpret_cast<const uint4 *>((which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + tile * tile_bytes + skip) + at);
+                        s[u] = (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile];
+                        dst[u] = (T *)(which ? a.v : a.k) + (first + shift + tok) * stride + (int64_t)h * D + (at - tok * vecs) * V;
+                        if (c0 + u * step >= all || e >= total) dst[u] = nullptr;
+                    }
+    #pragma unroll
+                    for (int u = 0; u < kLoadFlight; ++u) {
+                        if (!dst[u]) continue;
+                        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+                        Piece<T, V> out;
+    #pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float4 f = decode4<CODE>(w[j]);
+                            out.set2(4 * j, f.x * s[u], f.y * s[u]);
+                            out.set2(4 * j + 2, f.z * s[u], f.w * s[u]);
                         }
+                        out.store(dst[u]);
                     }
                 } else {
-                    for (int e = lane; e < total; e += 32) dst[(e / vecs) * stride + e % vecs] = rounded<T>(decode1<CODE>(tile[e]) * s);
+                    for (int c = c0; c < min(c0 + kLoadFlight * step, all); c += step) {
+                        const int item = c / chunks, e = (c - item * chunks) * 32 + lane, h = item >> 1, which = item & 1;
+                        if (e >= total) continue;
+                        const int64_t tile = tile0 + h;
+                        const float s = (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile];
+                        const uint8_t code = ((which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + tile * tile_bytes + skip)[e];
+                        ((T *)(which ? a.v : a.k))[(first + shift + e / vecs) * (which ? a.v_stride : a.k_stride) + (int64_t)h * D + e % vecs] =
+                            rounded<T>(decode1<CODE>(code) * s);
+                    }
                 }
             }
         }
@@ -325,7 +355,8 @@ __global__ void __launch_bounds__(kItemWarps * 32) load_q8_kernel(const __grid_c
 // Whether rows and pool allow 16 elements (32 bytes and more) and 16 codes at once.
 static bool wide_ok(const PoolViewQ8 &pv, const void *k, const void *v, int64_t k_stride, int64_t v_stride, int dtype) {
     const int64_t size = dtype_bytes(dtype);
-    if (pv.head_dim % 16 != 0) return false;
+    if (std::max(k_stride, v_stride) * pv.block_size >= (1ll << 31)) return false;   // (a page's rows are addressed in 32 bits)
+    if (pv.head_dim % 16 != 0 || pv.head_dim < 32) return false;
     if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * size) | (uintptr_t)(v_stride * size)) & 31) != 0) return false;
     for (int i = 0; i < pv.num_segments; ++i)
         if ((((uintptr_t)pv.k_base[i] | (uintptr_t)pv.v_base[i]) & 15) != 0) return false;
@@ -354,8 +385,11 @@ static int check_rows(const PoolViewQ8 &pv, int64_t k_stride, int64_t v_stride, 
     return k_stride < row || v_stride < row ? MKV_ERR_SHAPE : MKV_OK;
 }
 
-static int item_warps(const PoolViewQ8 &pv) { return std::min(2 * pv.num_kv_heads, kItemWarps); }
-static unsigned item_blocks(const PoolViewQ8 &pv) { return (unsigned)std::min<int64_t>(ceil_div64(2 * pv.num_kv_heads, kItemWarps), 65535); }
+// Warps of a block and blocks that share `items` of a page.
+static int warps_for(int items, int most) { return std::min(items, most); }
+static unsigned blocks_for(int items, int most) { return (unsigned)std::min<int64_t>(ceil_div64(items, most), 65535); }
+// e / n = umulhi(e, magic) for e n < 2^32: a page has at most 2^24 elements.  (n = 1 has no such factor; wide_ok keeps it out.)
+static uint32_t magic_of(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0u; }
 
 }  // namespace mkv
 
@@ -373,15 +407,17 @@ int mkv_store_kv_q8_prefill(int device, void *stream, const void *k, const void 
     if (num_seqs < 0 || max_seq_len < 0 || table_stride < 1 || num_rows < 0 || num_tokens < 0) return MKV_ERR_SHAPE;
     if ((st = check_rows(a.pool, k_stride, v_stride, dtype))) return st;
     if (cur_layer < 0 || cur_layer >= a.pool.num_layers) return MKV_ERR_RANGE;
-    if (num_seqs == 0 || max_seq_len == 0) return MKV_OK;
+    if (num_seqs == 0 || max_seq_len == 0 || num_tokens == 0) return MKV_OK;
     if (!k || !v || !block_table || !seq_ids || !seq_lens || !start_locs) return MKV_ERR_NULL;
     a.k = k; a.v = v; a.k_stride = k_stride; a.v_stride = v_stride; a.num_tokens = num_tokens;
     a.block_table = block_table; a.table_cols = table_stride; a.num_rows = num_rows;
     a.seq_ids = seq_ids; a.start_locs = start_locs; a.seq_lens = seq_lens; a.num_seqs = num_seqs; a.cur_layer = cur_layer;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return set_cuda_error(guard.err);
-    const dim3 grid((unsigned)ceil_div64(max_seq_len, a.pool.block_size), (unsigned)std::min(num_seqs, 65535), item_blocks(a.pool));
-    const int threads = item_warps(a.pool) * 32;
+    const dim3 grid((unsigned)ceil_div64(max_seq_len, a.pool.block_size), (unsigned)std::min(num_seqs, 65535),
+                    blocks_for(a.pool.num_kv_heads, kHeadWarps));
+    const int threads = warps_for(a.pool.num_kv_heads, kHeadWarps) * 32;
+    a.vecs_magic = magic_of(a.pool.head_dim / 16);
     const int64_t pieces = a.pool.tile_bytes / 16;
     dispatch(dtype, a.pool.code, wide_ok(a.pool, k, v, k_stride, v_stride, dtype), [&](auto t, auto code, auto w) {
         using T = decltype(t);
@@ -413,10 +449,11 @@ int mkv_store_kv_q8_decode(int device, void *stream, const void *k, const void *
     a.seq_ids = seq_ids; a.start_locs = nullptr; a.seq_lens = seq_lens; a.num_seqs = batch; a.cur_layer = cur_layer;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return set_cuda_error(guard.err);
-    const dim3 grid((unsigned)batch, item_blocks(a.pool));
+    const dim3 grid((unsigned)batch, blocks_for(2 * a.pool.num_kv_heads, kItemWarps));
+    a.vecs_magic = 0;
     dispatch(dtype, a.pool.code, wide_ok(a.pool, k, v, k_stride, v_stride, dtype), [&](auto t, auto code, auto w) {
         store_q8_decode_kernel<decltype(t), decltype(code)::value, decltype(w)::value>
-            <<<grid, item_warps(a.pool) * 32, 0, (cudaStream_t)stream>>>(a);
+            <<<grid, warps_for(2 * a.pool.num_kv_heads, kItemWarps) * 32, 0, (cudaStream_t)stream>>>(a);
     });
     MKV_LAUNCH_CHECK();
     return MKV_OK;
@@ -440,11 +477,22 @@ int mkv_load_kv_q8(int device, void *stream, void *k, void *v, int64_t k_stride,
     a.num_seqs = num_seqs; a.cur_layer = cur_layer;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return set_cuda_error(guard.err);
-    // a range that starts inside a block touches one block more
-    const dim3 grid((unsigned)(ceil_div64(max_len, a.pool.block_size) + 1), (unsigned)std::min(num_seqs, 65535), item_blocks(a.pool));
-    dispatch(dtype, a.pool.code, wide_ok(a.pool, k, v, k_stride, v_stride, dtype), [&](auto t, auto code, auto w) {
+    const bool wide = wide_ok(a.pool, k, v, k_stride, v_stride, dtype);
+    a.vecs_magic = magic_of(a.pool.head_dim / 16);
+    // A range that starts inside a block touches one block more.  A page's chunks go to so many blocks that a warp has eight
+    // of them (two flights), or four (one) where the ranges are a part of a page each or there would be few blocks otherwise
+    // (append and load back of 256 last pages: 10.2 us with four, 12.9 with eight, 13.6 with two; 32 prefixes of up to 2048 tokens:
+    // 25, 23, 28 us).
+    int sms = 0;
+    if ((st = mkv_sm_count(device, &sms))) return st;
+    const int64_t pages = num_out_rows / a.pool.block_size + 2 * (int64_t)num_seqs;
+    const int64_t chunks = ceil_div64(a.pool.tile_bytes / (wide ? 16 : 1), 32) * 2 * a.pool.num_kv_heads;
+    const int64_t rounds = num_out_rows >= (int64_t)num_seqs * a.pool.block_size && chunks * pages >= 8 * (kLoadThreads / 32) * 4ll * sms ? 8 : 4;
+    const dim3 grid((unsigned)(ceil_div64(max_len, a.pool.block_size) + 1), (unsigned)std::min(num_seqs, 65535),
+                    (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks / (rounds * (kLoadThreads / 32)), 65535)));
+    dispatch(dtype, a.pool.code, wide, [&](auto t, auto code, auto w) {
         load_q8_kernel<decltype(t), decltype(code)::value, decltype(w)::value>
-            <<<grid, item_warps(a.pool) * 32, 0, (cudaStream_t)stream>>>(a);
+            <<<grid, kLoadThreads, 0, (cudaStream_t)stream>>>(a);
     });
     MKV_LAUNCH_CHECK();
     return MKV_OK;
