@@ -156,30 +156,32 @@ __device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32
 }
 
 // int8 codes as fp16: the byte with its sign bit flipped is q + 128; set behind the byte 0x64 it is the fp16 number
-// 1024 + 128 + q.  K keeps the offset - the score's accumulator starts at -1152 sum(q) instead of 0, which costs at most
+// 1024 + 128 + q.  (One logic instruction for a word's even bytes, a byte permutation and one for the odd ones: 83.3 us on the
+// 256-sequence batch; with a shift in its place 87, with a multiplication 94: these instructions are what bounds the kernel there.)  K keeps the offset - the score's accumulator starts at -1152 sum(q) instead of 0, which costs at most
 // 1152 sum|q| 2^-22 in a score, less than summing 128 products in 32 bits may - while V's is taken off: a sum of weights
 // over a long context would bury the result under it.
 constexpr float kCodeOffset = 1152.f;
 
-// K: codes (0, 1) and (2, 3) of a word.
+
+// Codes (0, 2) and (1, 3) of a word: for K two dims each, whose order inside the k axis is the query's too; for V two tokens
+// of one dim, then of the next.  `c`: 0x00ff00ff and 0x64806480 in registers, so that (w & c.x) ^ c.y is one instruction (an
+// instruction has room for one constant, and the compiler makes two of it).
 template <int CODE>
-__device__ __forceinline__ void widen_k(uint32_t w, uint32_t &lo, uint32_t &hi) {
+__device__ __forceinline__ void widen_k(uint32_t w, uint2 c, uint32_t &even, uint32_t &odd) {
     if (CODE == MKV_Q8_INT8) {
-        const uint32_t x = w ^ 0x80808080u;
-        lo = __byte_perm(x, 0x64646464u, 0x4140);
-        hi = __byte_perm(x, 0x64646464u, 0x4342);
+        asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n" : "=r"(even) : "r"(w), "r"(c.x), "r"(c.y));
+        odd = __byte_perm(w, 0u, 0x4341) ^ c.y;
     } else {
-        e4m3x4_to_half2(w, lo, hi);
+        e4m3x4_to_half2(w, even, odd);      // (0, 1) and (2, 3): K's dims as they stand
     }
 }
-// V: codes (0, 2) and (1, 3) of a word: two tokens of one dim, then of the next.
 template <int CODE>
-__device__ __forceinline__ void widen_v(uint32_t w, uint32_t &even, uint32_t &odd) {
+__device__ __forceinline__ void widen_v(uint32_t w, uint2 c, uint32_t &even, uint32_t &odd) {
     if (CODE == MKV_Q8_INT8) {
-        const uint32_t x = w ^ 0x80808080u;
         const __half2 off = __float2half2_rn(-kCodeOffset);
-        even = half2_bits(__hadd2(bits_half2(__byte_perm(x, 0x64646464u, 0x4240)), off));
-        odd = half2_bits(__hadd2(bits_half2(__byte_perm(x, 0x64646464u, 0x4341)), off));
+        widen_k<CODE>(w, c, even, odd);
+        even = half2_bits(__hadd2(bits_half2(even), off));
+        odd = half2_bits(__hadd2(bits_half2(odd), off));
     } else {
         e4m3x4_to_half2(__byte_perm(w, 0u, 0x3120), even, odd);
     }
@@ -485,6 +487,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     const uint32_t v_at = 2 * HB + (D == 128 ? vr * 128 + ((vh ^ (vr & 7)) << 4)
                                              : (vr >> 1) * 128 + ((((vr & 1) * 4 + vh) ^ ((vr >> 1) & 3)) << 4));
 
+    uint2 masks;
+    asm volatile("mov.b32 %0, 0x00ff00ff;\nmov.b32 %1, 0x64806480;\n" : "=r"(masks.x), "=r"(masks.y));
+
     bool busy = more;
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) {
@@ -552,8 +557,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 }
 #pragma unroll
                 for (int i = 0; i < KW; ++i) {
-                    qf[n][i][0] = raw[2 * i];
-                    qf[n][i][1] = raw[2 * i + 1];
+                    // dims 4 i ... 4 i + 3 in the order in which widen_k() has them
+                    qf[n][i][0] = CODE == MKV_Q8_INT8 ? __byte_perm(raw[2 * i], raw[2 * i + 1], 0x5410) : raw[2 * i];
+                    qf[n][i][1] = CODE == MKV_Q8_INT8 ? __byte_perm(raw[2 * i], raw[2 * i + 1], 0x7632) : raw[2 * i + 1];
                 }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
@@ -587,8 +593,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t a0, a1, a2, a3;
-                        widen_k<CODE>(xs[j], a0, a2);
-                        widen_k<CODE>(ys[j], a1, a3);
+                        widen_k<CODE>(xs[j], masks, a0, a2);
+                        widen_k<CODE>(ys[j], masks, a1, a3);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) mma(part[n][j & 1], a0, a1, a2, a3, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
                     }
@@ -671,8 +677,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
                     uint32_t a0, a1, a2, a3;
-                    widen_v<CODE>(w[2 * d], a0, a1);
-                    widen_v<CODE>(w[2 * d + 1], a2, a3);
+                    widen_v<CODE>(w[2 * d], masks, a0, a1);
+                    widen_v<CODE>(w[2 * d + 1], masks, a2, a3);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma(o[n][c + d], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                 }
