@@ -38,22 +38,19 @@ def alloc_kvcache_q8(num_blocks: int, model_config, engine_config, dtype: torch.
     return (*codes, *[torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)])
 
 
-# mkv_pool_q8, packed rather than assigned field by field: the header, then one pointer of each kind a segment.
-_HEADER = struct.Struct("6i2q")
-_POINTER = struct.Struct("Q")
+# mkv_pool_q8, packed rather than assigned field by field: the header and the first segment's four pointers at once (each
+# stands in front of an array), further segments' pointers one by one.
 _FIELDS = (MkvPoolQ8.k_base.offset, MkvPoolQ8.v_base.offset, MkvPoolQ8.k_scale.offset, MkvPoolQ8.v_scale.offset)
+_PACK = struct.Struct("6i2qQ%dxQ%dxQ%dxQ" % tuple(y - x - 8 for x, y in zip(_FIELDS, _FIELDS[1:]))).pack_into
+_POINTER = struct.Struct("Q").pack_into
 
 
-def _segment(buf, i, k, v, ks, vs, dtype, shape, dev):
-    assert k.shape == shape and v.shape == shape and ks.shape == shape[:3] and vs.shape == shape[:3]
+def _check_segment(k, v, ks, vs, dtype, shape, entries, dev):
+    assert k.shape == shape and v.shape == shape and ks.numel() == entries and vs.numel() == entries, \
+        "k_cache and v_cache have one shape, the scales one entry for each block, layer and head"
     assert k.dtype is dtype and v.dtype is dtype and ks.dtype is torch.float32 and vs.dtype is torch.float32
     assert k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
     assert k.get_device() == dev and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev
-    at = 8 * i
-    _POINTER.pack_into(buf, _FIELDS[0] + at, k.data_ptr())
-    _POINTER.pack_into(buf, _FIELDS[1] + at, v.data_ptr())
-    _POINTER.pack_into(buf, _FIELDS[2] + at, ks.data_ptr())
-    _POINTER.pack_into(buf, _FIELDS[3] + at, vs.data_ptr())
 
 
 def _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new, model_config,
@@ -66,25 +63,27 @@ def _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_
     code = _CODES.get(dtype)
     if code is None:
         raise RuntimeError(f"unsupported 8-bit KV dtype {dtype}")
-    n_new = len(k_cache_new)
-    if n_new + 1 > MKV_MAX_SEGMENTS:
-        raise RuntimeError(f"too many elastic KV chunks ({n_new}); the library supports {MKV_MAX_SEGMENTS - 1}")
-    assert len(v_cache_new) == n_new and len(k_scale_new) == n_new and len(v_scale_new) == n_new
     blocks, layers, heads, bs, d = shape
     assert heads == model_config.num_kv_heads and d == model_config.head_dim and bs == engine_config.block_size
-    buf = MkvPoolQ8()
-    _segment(buf, 0, k_cache, v_cache, k_scale, v_scale, dtype, shape, dev)
+    _check_segment(k_cache, v_cache, k_scale, v_scale, dtype, shape, blocks * layers * heads, dev)
+    n_new = len(k_cache_new)
+    assert len(v_cache_new) == n_new and len(k_scale_new) == n_new and len(v_scale_new) == n_new
+    pool = MkvPoolQ8()
+    _PACK(pool, 0, 1 + n_new, code, layers, heads, bs, d, blocks, int(chunk_blocks) if n_new else 0, k_cache.data_ptr(),
+          v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
     if n_new:
+        if n_new + 1 > MKV_MAX_SEGMENTS:
+            raise RuntimeError(f"too many elastic KV chunks ({n_new}); the library supports {MKV_MAX_SEGMENTS - 1}")
         if int(num_blocks_org) != blocks:
             raise RuntimeError("num_blocks_org is not the number of blocks of the original pool")
-        chunk_blocks = int(chunk_blocks)
-        chunk = torch.Size((chunk_blocks, layers, heads, bs, d))
-        for j in range(n_new):
-            if k_cache_new[j].shape != chunk:
+        chunk = torch.Size((int(chunk_blocks), layers, heads, bs, d))
+        for j, parts in enumerate(zip(k_cache_new, v_cache_new, k_scale_new, v_scale_new)):
+            if parts[0].shape != chunk:
                 raise RuntimeError("elastic KV chunks must all hold kv_cache_new_block_size blocks of the pool's shape")
-            _segment(buf, 1 + j, k_cache_new[j], v_cache_new[j], k_scale_new[j], v_scale_new[j], dtype, chunk, dev)
-    _HEADER.pack_into(buf, 0, 1 + n_new, code, layers, heads, bs, d, blocks, chunk_blocks if n_new else 0)
-    return buf, shape, dev
+            _check_segment(*parts, dtype, chunk, chunk[0] * layers * heads, dev)
+            for field, t in zip(_FIELDS, parts):
+                _POINTER(pool, field + 8 * (1 + j), t.data_ptr())
+    return pool, shape, dev
 
 
 def _rows(x, heads, d, dev):
