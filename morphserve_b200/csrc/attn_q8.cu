@@ -155,16 +155,18 @@ __device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32
     asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 
-// int8 codes as fp16: the byte with its sign bit flipped is q + 128; set behind the byte 0x64 it is the fp16 number
-// 1024 + 128 + q.  (One logic instruction for a word's even bytes, a byte permutation and one for the odd ones: 83.3 us on the
-// 256-sequence batch; with a shift in its place 87, with a multiplication 94: these instructions are what bounds the kernel there.)  K keeps the offset - the score's accumulator starts at -1152 sum(q) instead of 0, which costs at most
-// 1152 sum|q| 2^-22 in a score, less than summing 128 products in 32 bits may - while V's is taken off: a sum of weights
-// over a long context would bury the result under it.
-constexpr float kCodeOffset = 1152.f;
-
+// int8 codes as fp16: the byte with its sign bit flipped is u = q + 128, and as the low byte of an fp16 number it IS u 2^-24,
+// a subnormal number, which the tensor core takes as it stands - no arithmetic at all.  The 128 leaves inside the products:
+// the score's accumulator starts at -128 sum(q_i) instead of 0, and -128 times the weights are added to O by a product with a
+// constant tile, half by half, so that sums over a long context are not buried under it (128 sum|x| 2^-23 at most, less than
+// summing as many products in 32 bits may cost anyway).  2^24 goes into the scale of the scores and the last division.
+// (As 1024 + u with the offset taken off by 32 additions a half instead, the 256-sequence batch took 82.9 us instead of 81.7.)
+constexpr float kCodeUnit = 16777216.f;             // 2^24
+constexpr float kCodeOffset = 128.f / 16777216.f;
+constexpr uint32_t kMinusOffset2 = 0x80808080u;     // two fp16 numbers -128 2^-24
 
 // Codes (0, 2) and (1, 3) of a word: for K two dims each, whose order inside the k axis is the query's too; for V two tokens
-// of one dim, then of the next.  `c`: 0x00ff00ff and 0x64806480 in registers, so that (w & c.x) ^ c.y is one instruction (an
+// of one dim, then of the next.  `c`: 0x00ff00ff and 0x00800080 in registers, so that (w & c.x) ^ c.y is one instruction (an
 // instruction has room for one constant, and the compiler makes two of it).
 template <int CODE>
 __device__ __forceinline__ void widen_k(uint32_t w, uint2 c, uint32_t &even, uint32_t &odd) {
@@ -177,14 +179,8 @@ __device__ __forceinline__ void widen_k(uint32_t w, uint2 c, uint32_t &even, uin
 }
 template <int CODE>
 __device__ __forceinline__ void widen_v(uint32_t w, uint2 c, uint32_t &even, uint32_t &odd) {
-    if (CODE == MKV_Q8_INT8) {
-        const __half2 off = __float2half2_rn(-kCodeOffset);
-        widen_k<CODE>(w, c, even, odd);
-        even = half2_bits(__hadd2(bits_half2(even), off));
-        odd = half2_bits(__hadd2(bits_half2(odd), off));
-    } else {
-        e4m3x4_to_half2(__byte_perm(w, 0u, 0x3120), even, odd);
-    }
+    if (CODE == MKV_Q8_INT8) widen_k<CODE>(w, c, even, odd);
+    else e4m3x4_to_half2(__byte_perm(w, 0u, 0x3120), even, odd);
 }
 
 template <typename T>
@@ -488,7 +484,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                                              : (vr >> 1) * 128 + ((((vr & 1) * 4 + vh) ^ ((vr >> 1) & 3)) << 4));
 
     uint2 masks;
-    asm volatile("mov.b32 %0, 0x00ff00ff;\nmov.b32 %1, 0x64806480;\n" : "=r"(masks.x), "=r"(masks.y));
+    asm volatile("mov.b32 %0, 0x00ff00ff;\nmov.b32 %1, 0x00800080;\n" : "=r"(masks.x), "=r"(masks.y));
 
     bool busy = more;
 #pragma unroll
@@ -574,7 +570,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         for (int h = 0; h < 2; ++h) {
             const uint32_t at = st + h * HB;
             const int tokens = (int)((ma.x >> (8 + 8 * h)) & 0xffu);
-            const float ks = __uint_as_float(h ? scales.y : scales.x), vs = __uint_as_float(h ? scales.w : scales.z);
+            const float ks = __uint_as_float(h ? scales.y : scales.x) * (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f), vs = __uint_as_float(h ? scales.w : scales.z);
             // ---- S^T = K Q^T
             float sc[NT][4];
             {
@@ -665,6 +661,13 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
             // ---- O^T += V^T P^T: row tile c has dim 16 c + 2 g in its row g and dim 16 c + 2 g + 1 in its row g + 8
             // Behind the sequence's end any byte may stand, an e4m3 NaN among them, and 0 x NaN is NaN.
             const bool cut = CODE == MKV_Q8_E4M3 && tokens < kHalf;
+            if (CODE == MKV_Q8_INT8) {
+#pragma unroll
+                for (int c = 0; c < MT; ++c)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        mma(o[n][c], kMinusOffset2, kMinusOffset2, kMinusOffset2, kMinusOffset2, pb[n][0], pb[n][1]);
+            }
 #pragma unroll
             for (int c = 0; c < MT; c += 2) {
                 uint32_t w[4];      // (16-dim piece c: tokens 0-7, 8-15; piece c + 1: the same)
@@ -727,12 +730,12 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     const int head = n * 8 + 2 * t + e;
                     if (head >= heads || head >= HC) continue;
                     if (whole) {
-                        const float f = 1.f / l[n][e];
+                        const float f = (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f) / l[n][e];
                         T *dst = (T *)p.o + ((int64_t)b * p.num_q_heads + hq0 + head) * D + 2 * g;
 #pragma unroll
                         for (int i = 0; i < MT; ++i) store2<T>(dst + 16 * i, o[n][i][e] * f, o[n][i][e + 2] * f);
                     } else {
-                        const float f = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+                        const float f = l[n][e] == 0.f ? 0.f : (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f) / l[n][e];
                         float *dst = row + head * D + 2 * g;
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
