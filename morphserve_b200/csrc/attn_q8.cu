@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     bool bad = false, more = false;
     int cb = 0, chp = 0, ch = 0, chg = 0, cnt = 0, cj = 0, cjend = 0, clen = 0, crow = 0, cbase = 0, crem = 0;
     int first_flag = 1;
-    uint64_t uoff = 0;              // bytes of the unit's (layer, head) inside a block's codes
+    uint32_t uhead = 0;             // the unit's (layer, head) inside a block ...
+    uint64_t ubase = 0;             // ... and where this lane's first piece of it stands in the block's codes
     int2 ids, ids_next;             // lane l: block ids of tile cbase + l's halves, and of the 32 tiles behind those
     int2 ids0_next = make_int2(-1, -1);  // ... of the first 32 tiles of the next sequence (nb; its row and length)
     int nb = -2, nrow = 0, nlen = 0;    // -1: there is none, -2: not looked for yet
@@ -340,7 +341,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         clen = min(clen, p.max_len);
     };
     auto enter_head = [&]() {
-        uoff = (uint64_t)(uint32_t)(p.cur_layer * p.num_kv_heads + ch) * p.tile_bytes;
+        uhead = (uint32_t)(p.cur_layer * p.num_kv_heads + ch);
+        ubase = (uint64_t)uhead * p.tile_bytes + (uint32_t)lane * 16;
         cjend = min(cnt, crem);
         more = cj < cjend;
         cbase = cj;
@@ -378,7 +380,6 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         ids = load_ids(crow, cj, cnt);
         enter_head();
     }
-    const uint64_t lane16 = (uint64_t)lane * 16;
     const uint32_t block_bytes = p.tile_bytes * p.block_tiles;
     // 16-byte piece i * 32 + lane of a half.  D = 128: piece c of token r goes to c ^ (r & 7); D = 64: two tokens share a
     // 128-byte line, whose pieces go to c ^ (line & 3).  Either way the reads below meet no conflict.
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 v0 = p.pool.v_base[seg];
                 s0 = lane ? p.pool.v_scale[seg] : p.pool.k_scale[seg];
             }
-            const uint64_t off = (uint64_t)row * block_bytes + uoff + (uint32_t)(((2 * cj + h) & half_mask) * HB) + lane16;
+            const uint64_t off = (uint64_t)row * block_bytes + ubase + (uint32_t)(((2 * cj + h) & half_mask) * HB);
             const uint8_t *kt = k0 + off, *vt = v0 + off;
 #pragma unroll
             for (int i = 0; i < HB / 512; ++i) {
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 cp16(to + 2 * HB, vt + i * 512);
             }
             if (lane < 2)
-                cp4(st + META + (lane * 2 + h) * 4, s0 + ((uint64_t)row * p.block_tiles + (uint32_t)(p.cur_layer * p.num_kv_heads + ch)));
+                cp4(st + META + (lane * 2 + h) * 4, s0 + ((uint64_t)row * p.block_tiles + uhead));
         } else {
             bad |= tokens > 0;
             tokens = 0;
@@ -425,8 +426,24 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         const uint32_t blk1 = (uint32_t)__shfl_sync(0xffffffffu, ids.y, cj - cbase);
         const int left = clen - cj * kTile;
         int n0 = min(left, kHalf), n1 = min(max(left - kHalf, 0), kHalf);
-        issue_half(st, 0, blk0, n0);
-        issue_half(st, 1, blk1, n1);
+        if (n1 > 0 && max(blk0, blk1) < p.total_blocks && p.num_segments == 1) {    // both halves, as nearly always
+            const uint32_t sub0 = (uint32_t)((2 * cj & half_mask) * HB), sub1 = (uint32_t)(((2 * cj + 1) & half_mask) * HB);
+            const uint64_t off0 = (uint64_t)blk0 * block_bytes + sub0 + ubase, off1 = (uint64_t)blk1 * block_bytes + sub1 + ubase;
+            const uint8_t *k0 = p.k0 + off0, *v0 = p.v0 + off0, *k1 = p.k0 + off1, *v1 = p.v0 + off1;
+#pragma unroll
+            for (int i = 0; i < HB / 512; ++i) {
+                const uint32_t to = st + i * 512 + (D == 128 && (i & 1) ? put ^ 64 : put);
+                cp16(to, k0 + i * 512);
+                cp16(to + HB, k1 + i * 512);
+                cp16(to + 2 * HB, v0 + i * 512);
+                cp16(to + 3 * HB, v1 + i * 512);
+            }
+            if (lane < 4)
+                cp4(st + META + lane * 4, (lane & 2 ? p.vs0 : p.ks0) + ((uint64_t)(lane & 1 ? blk1 : blk0) * p.block_tiles + uhead));
+        } else {
+            issue_half(st, 0, blk0, n0);
+            issue_half(st, 1, blk1, n1);
+        }
         if (first_flag) {       // the unit's query rows on their way into the cache
             const int hq0 = ch * p.group + chg * HC, bytes = min(HC, p.group - chg * HC) * D * 2;
             if (lane * 128 < bytes)
@@ -573,32 +590,22 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
             const float ks = __uint_as_float(h ? scales.y : scales.x) * (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f), vs = __uint_as_float(h ? scales.w : scales.z);
             // ---- S^T = K Q^T
             float sc[NT][4];
-            {
-                float part[NT][2][4];   // two chains, for the latency
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        part[n][0][e] = CODE == MKV_Q8_INT8 ? kinit[n][e & 1] : 0.f;
-                        part[n][1][e] = 0.f;
-                    }
+                for (int e = 0; e < 4; ++e) sc[n][e] = CODE == MKV_Q8_INT8 ? kinit[n][e & 1] : 0.f;
 #pragma unroll
-                for (int i = 0; i < KW / 4; ++i) {
-                    const uint4 x = lds16(at + (k_at ^ (i << 4))), y = lds16(at + (k_at ^ (i << 4)) + HB / 2);  // tokens g and g + 8
-                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+            for (int i = 0; i < KW / 4; ++i) {
+                const uint4 x = lds16(at + (k_at ^ (i << 4))), y = lds16(at + (k_at ^ (i << 4)) + HB / 2);  // tokens g and g + 8
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t a0, a1, a2, a3;
-                        widen_k<CODE>(xs[j], masks, a0, a2);
-                        widen_k<CODE>(ys[j], masks, a1, a3);
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t a0, a1, a2, a3;
+                    widen_k<CODE>(xs[j], masks, a0, a2);
+                    widen_k<CODE>(ys[j], masks, a1, a3);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma(part[n][j & 1], a0, a1, a2, a3, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
-                    }
+                    for (int n = 0; n < NT; ++n) mma(sc[n], a0, a1, a2, a3, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[n][e] = part[n][0][e] + part[n][1][e];
             }
             // ---- softmax: token g (elements 0, 1) and g + 8 (2, 3), heads 2t, 2t + 1
             // The block's V scale joins the exponent: weights are 2^(score + log2 s_v - base), so that O accumulates across
