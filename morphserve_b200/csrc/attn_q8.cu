@@ -151,9 +151,6 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
-__device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
-}
 
 // int8 codes as fp16: the byte with its sign bit flipped is u = q + 128, and as the low byte of an fp16 number it IS u 2^-24,
 // a subnormal number, which the tensor core takes as it stands - no arithmetic at all.  The 128 leaves inside the products:

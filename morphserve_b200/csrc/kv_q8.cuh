@@ -98,10 +98,9 @@ __device__ __forceinline__ uint8_t encode1(float a, float inv) {
 }
 
 // ---- codes to numbers -----------------------------------------------------------------------------------------
-// Two e4m3 codes (low 16 bits) as fp16: exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four e4m3 codes as fp16: exact.
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 template <int CODE>
 __device__ __forceinline__ float decode1(uint32_t byte) {
@@ -110,9 +109,16 @@ __device__ __forceinline__ float decode1(uint32_t byte) {
 }
 template <int CODE>
 __device__ __forceinline__ float4 decode4(uint32_t w) {
-    if (CODE == MKV_Q8_INT8)
-        return make_float4((float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24));
-    const uint32_t lo = e4m3x2_to_half2(w & 0xffffu), hi = e4m3x2_to_half2(w >> 16);
+    uint32_t lo, hi;
+    if (CODE == MKV_Q8_INT8) {  // behind the byte 0x64 a code with its sign bit flipped is the fp16 number 1024 + 128 + q
+        const uint32_t x = w ^ 0x80808080u, y = __byte_perm(x, 0x64646464u, 0x4140), z = __byte_perm(x, 0x64646464u, 0x4342);
+        const __half2 off = __float2half2_rn(-1152.f), l = __hadd2(*reinterpret_cast<const __half2 *>(&y), off),
+                      h = __hadd2(*reinterpret_cast<const __half2 *>(&z), off);
+        lo = *reinterpret_cast<const uint32_t *>(&l);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        e4m3x4_to_half2(w, lo, hi);
+    }
     const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&lo)), b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
     return make_float4(a.x, a.y, b.x, b.y);
 }
