@@ -108,7 +108,7 @@ class KVCacheModelState:
         if self._cos_cached is None:
             self._init_to_get_rotary()
         seq_block_size, num_seq_blocks = seq_block_size_heuristic(mc.num_kv_heads, decoding_seq_lens_list)
-        return LlamaInferState(
+        state = LlamaInferState(
             batch_size=batch, num_tokens=n_tok, seq_ids=seq_ids, softmax_scale=mc.head_dim ** -0.5,
             num_prefill_seqs=n_pre, num_prefill_tokens=n_pre_tok, prefill_seq_start_locs=starts_with_end[:n_pre],
             prefill_seq_start_locs_with_end=starts_with_end, prefill_seq_lens=seq_lengths[:n_pre],
@@ -119,6 +119,8 @@ class KVCacheModelState:
             kv_cache_new_block_size=self.kv_cache_new_block_size, org_layer_param_size=self.org_layer_param_size,
             position_cos=self._cos_cached[positions], position_sin=self._sin_cached[positions],
             ignore_kvcache=ignore_kvcache)
+        state.positions = positions     # int32 [num_tokens], for rotary_embedding_positions; not a field of the reference's class
+        return state
 
     @torch.inference_mode()
     def init_kvcache_and_swap(self, num_blocks: int):

@@ -509,3 +509,75 @@ def test_python_refusals_on_the_gpu(mk):
         c.attend(mk, q[:1], st)
     with pytest.raises(RuntimeError):
         mk.paged_attention_q8(q, *pool, c.table_t, c.mc, c.ec, st, 2, torch.zeros((2, c.hq * c.d), dtype=torch.float16, device="cuda"))
+
+
+def test_steps_of_the_model_state_on_an_8_bit_pool(mk):
+    """The framework's own step - block manager, lengths and positions from prepare_step - over an 8-bit pool, with a chunk
+    added to it half way."""
+    mc = types.SimpleNamespace(num_layers=2, num_q_heads=8, num_kv_heads=2, head_dim=64, max_position_embeddings=256)
+    ec = types.SimpleNamespace(block_size=16, max_blocks_per_seq=8, max_seqs_in_block_table=6, num_cpu_blocks=2)
+    state = mk.KVCacheModelState(mc, ec)
+    state.gpu_block_manager = mk.BlockManager("GPU", 12, 6, 8, 16)
+    pool = [mk.alloc_kvcache_q8(12, mc, ec, torch.int8)]
+    c = Case("int8", [1], hq=8, hkv=2, d=64, layers=2, layer=1, seed=30)
+    as_numpy = lambda p: dict(k=p[0].view(torch.uint8).cpu().numpy(), v=p[1].view(torch.uint8).cpu().numpy(),  # noqa: E731
+                              ks=p[2].cpu().numpy(), vs=p[3].cpu().numpy())
+    c.segs = [as_numpy(pool[0])]
+    inv, att = mk.rotary_inv_freq(mc)
+    lens = {3: 17, 0: 5}
+    for i in range(30):
+        order = list(lens)
+        if i == 0:
+            st = state.prepare_step([[0] * n for n in lens.values()], order, [])
+        else:
+            for s in lens:
+                lens[s] += 1
+            st = state.prepare_step([[0]] * len(lens), order, list(lens.values()))
+        if i == 20:     # the pool grows, as an elastic expansion does it
+            pool.append(mk.alloc_kvcache_q8(4, mc, ec, torch.int8))
+            c.segs.append(as_numpy(pool[1]))
+        st.kv_cache_new_block_size = 4
+        n = st.num_tokens
+        want = [p for s in order for p in range(lens[s])] if i == 0 else [lens[s] - 1 for s in order]
+        assert st.positions.tolist() == want
+        qkv, _ = c.rows(n, 12, torch.float16)
+        q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
+        mk.rotary_embedding_positions(q, k, st.positions, inv, attention_scale=att)
+        table = state.gpu_block_manager.block_table
+        args = (*pool[0], [p[0] for p in pool[1:]], [p[1] for p in pool[1:]], [p[2] for p in pool[1:]], [p[3] for p in pool[1:]],
+                table, mc, ec, st, 1)
+        mk.store_kvcache_q8(k, v, *args)
+        kn, vn, c.table = k.double().cpu().numpy(), v.double().cpu().numpy(), table.cpu().numpy()
+        if i == 0:
+            O.store_prefill(c.segs, "int8", kn, vn, c.table, order, [0, 17], [17, 5], 1, 16)
+        else:
+            O.store_append(c.segs, "int8", kn, vn, c.table, order, list(lens.values()), 1, 16)
+            o = torch.zeros((2, 512), dtype=torch.float16, device="cuda")
+            mk.paged_attention_q8(q, *args, o)
+            c.check_attention(o, q.double().cpu().numpy(), lens=list(lens.values()), ids=order)
+    for p, s in zip(pool, c.segs):
+        assert np.array_equal(p[0].view(torch.uint8).cpu().numpy(), s["k"]) and np.array_equal(p[3].cpu().numpy(), s["vs"])
+
+
+def test_block_swap_of_an_8_bit_pool_as_views(mk):
+    """Codes as an fp16 pool of half the head dim, scales as an fp32 pool: out to the host and back, byte for byte."""
+    from morphserve_b200 import swiftllm_c
+    mc = types.SimpleNamespace(num_layers=2, num_kv_heads=4, head_dim=64)
+    pool = mk.alloc_kvcache_q8(10, mc, types.SimpleNamespace(block_size=16), torch.float8_e4m3fn)
+    for t in pool:
+        t.view(torch.uint8).random_(0, 256)
+    codes = [t.view(torch.float16) for t in pool[:2]]
+    scales = [t.view(10, 2, 4, 1, 1) for t in pool[2:]]
+    before = [t.view(torch.uint8).clone() for t in pool]
+    out = torch.tensor([7, 2, 9], dtype=torch.int64, device="cuda")
+    host = torch.tensor([0, 3, 1], dtype=torch.int64, device="cuda")
+    back = torch.tensor([1, 4, 0], dtype=torch.int64, device="cuda")
+    for pair in (codes, scales):
+        swap = [torch.zeros((4,) + tuple(t.shape[1:]), dtype=t.dtype).pin_memory() for t in pair]
+        swiftllm_c.swap_blocks(out, host, False, *pair, *swap)
+        torch.cuda.synchronize()
+        swiftllm_c.swap_blocks(host, back, True, *pair, *swap)
+    torch.cuda.synchronize()
+    for t, was in zip(pool, before):
+        now = t.view(torch.uint8)
+        assert torch.equal(now[back], was[out]) and torch.equal(now[[2, 3, 5, 6, 7, 8, 9]], was[[2, 3, 5, 6, 7, 8, 9]])
