@@ -356,7 +356,7 @@ int mkv_store_kv_prefill(int device, void *stream, const void *k, const void *v,
  * Decode: token len-1 of every sequence is appended.  In the first slot of a block its scale starts from the new token;
  * later the larger of the block's and the token's scale holds, and if that is the token's, the codes of the slots
  * before it are rounded again to the new scale (int8: q * fl32(old * fl32(1 / new)); e4m3: q * old / new).
- * A sequence given more than once: its last entry counts.  Sequences whose length is not positive, ids outside the
+ * A block that a call writes belongs to one sequence of it.  A sequence given more than once: its last entry counts.  Sequences whose length is not positive, ids outside the
  * table, positions behind the table's last column and blocks outside the pool are skipped.
  */
 int mkv_store_kv_q8_prefill(int device, void *stream, const void *k, const void *v, int64_t k_stride, int64_t v_stride,

@@ -15,6 +15,7 @@ int validate_pool_q8(const mkv_pool_q8 *pool, PoolViewQ8 *out) {
     if (pool->code != MKV_Q8_INT8 && pool->code != MKV_Q8_E4M3) return MKV_ERR_DTYPE;
     if (pool->num_layers < 1 || pool->num_kv_heads < 1 || pool->block_size < 1 || pool->head_dim < 1) return MKV_ERR_SHAPE;
     if ((int64_t)pool->block_size * pool->head_dim > (1 << 24)) return MKV_ERR_SHAPE;
+    if ((int64_t)pool->block_size * pool->head_dim * pool->num_kv_heads > (1 << 30)) return MKV_ERR_SHAPE;  // a page is counted in 32 bits
     if (pool->num_blocks_org < 0 || (pool->num_segments > 1 && pool->chunk_blocks < 1)) return MKV_ERR_SHAPE;
     PoolViewQ8 v;
     memset(&v, 0, sizeof(v));

@@ -198,7 +198,8 @@ extern "C" int mkv_rotary_positions(int device, void *stream, const void *q, con
     if (num_tokens < 0 || num_tokens > 0x7fffffff || num_q_heads < 0 || num_kv_heads < 0 || num_q_heads + num_kv_heads < 1 ||
         head_dim < 2 || num_pairs < 1 || 2 * num_pairs > head_dim || num_pairs > 2048)
         return MKV_ERR_SHAPE;
-    if ((int64_t)(num_q_heads + num_kv_heads) * head_dim > (1 << 26)) return MKV_ERR_SHAPE;
+    const int64_t all_heads = (int64_t)num_q_heads + num_kv_heads;
+    if (all_heads > 65535 || all_heads * head_dim > (1 << 26)) return MKV_ERR_SHAPE;     // (heads_magic is exact up to there)
     if (num_tokens == 0) return MKV_OK;
     if (!strides || !positions || !inv_freq) return MKV_ERR_NULL;
     if ((num_q_heads && (!q || !q_out)) || (num_kv_heads && (!k || !k_out))) return MKV_ERR_NULL;

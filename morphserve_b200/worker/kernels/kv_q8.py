@@ -136,9 +136,9 @@ def store_kvcache_q8(
 
     A prompt's blocks take their scales from the prompt alone (slots behind its end keep their bytes).  A decoding
     sequence's newest token is appended: in the first slot of a block the scale starts from it, later the larger of the
-    block's scale and the token's holds, and where that is the token's the older codes are rounded again.  A sequence
-    given more than once in one of the two parts: its last entry counts.  Sequences of length 0, ids outside the table
-    and blocks outside the pool are skipped."""
+    block's scale and the token's holds, and where that is the token's the older codes are rounded again.  A block that
+    a call writes belongs to one sequence: a scale has one writer.  A sequence given more than once in one of the two
+    parts: its last entry counts.  Sequences of length 0, ids outside the table and blocks outside the pool are skipped."""
     pool, shape, dev = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new,
                              model_config, engine_config, infer_state.num_blocks_org, infer_state.kv_cache_new_block_size)
     heads, d = shape[2], shape[4]

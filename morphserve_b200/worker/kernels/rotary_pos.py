@@ -32,7 +32,8 @@ def rotary_inv_freq(model_config, device="cuda"):
       llama3           by bands of turns over ``original_max_position_embeddings``: above ``high_freq_factor`` kept, below
                        ``low_freq_factor`` divided by ``factor``, blended between
       yarn             by pair index: kept above ``beta_fast`` (32) turns, divided below ``beta_slow`` (1), a ramp between;
-                       attention_scale = ``attention_factor``, else 0.1 ln(factor) + 1
+                       attention_scale = ``attention_factor``, else 0.1 ln(factor) + 1; its further variants (``mscale``,
+                       ``mscale_all_dim``, ``truncate`` switched off) are refused
     """
     dim = int(model_config.head_dim * (getattr(model_config, "partial_rotary_factor", 1.0) or 1.0))
     dim -= dim % 2
@@ -67,6 +68,8 @@ def rotary_inv_freq(model_config, device="cuda"):
             keep = ((original * inv / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
             inv = inv * keep + inv / factor * (1 - keep)
         else:
+            if scaling.get("mscale") or scaling.get("mscale_all_dim") or scaling.get("truncate", True) is False:
+                raise ValueError("yarn scaling with mscale, mscale_all_dim or truncate=False")
             at = [dim * math.log(original / (float(scaling.get(name, turns)) * 2 * math.pi)) / (2 * math.log(base))
                   for name, turns in (("beta_fast", 32.0), ("beta_slow", 1.0))]
             low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dim - 1)
@@ -86,7 +89,11 @@ def _strides(x, n, heads, d):
     """Distances of two tokens and of two heads; elements are contiguous, nothing overlaps."""
     s = x.stride()
     assert s[2] == 1, "elements are contiguous"
-    assert (n <= 1 or s[0] >= d) and (heads <= 1 or s[1] >= d), "tokens and heads do not overlap"
+    if n > 1 and heads > 1:     # the heads of a token lie in front of the next token, or the other way round
+        near, far, inner = (s[1], s[0], heads) if s[0] >= s[1] else (s[0], s[1], n)
+        assert near >= d and far >= (inner - 1) * near + d, "tokens and heads do not overlap"
+    else:
+        assert (n <= 1 or s[0] >= d) and (heads <= 1 or s[1] >= d), "tokens and heads do not overlap"
     return s
 
 

@@ -190,3 +190,31 @@ def test_rotary_c_entry_point_checks_its_arguments_on_the_host(mk):
     for bad in (dict(pairs=0), dict(pairs=33), dict(d=1), dict(n=-1), dict(hq=0, hkv=0), dict(hq=-1)):
         assert call(**bad) == -2, bad
     assert call(q=None) == -1 and call(pos=None) == -1 and call(inv=None) == -1 and call(strides=None) == -1
+
+
+def test_sizes_that_32_bits_do_not_count_are_refused(mk):
+    from morphserve_b200 import _lib as L
+    wide = _pool_q8(L, block_size=1 << 12, head_dim=1 << 12, num_kv_heads=65)     # 65 * 2^24 elements a page
+    assert L.lib.mkv_store_kv_q8_decode(0, None, 4096, 4096, 65 << 12, 65 << 12, 0, wide, 4096, 4, 4, 4096, 4096, 1, 0) == -2
+    strides = (C.c_int64 * 8)(*[2] * 8)
+    assert L.lib.mkv_rotary_positions(0, None, 4096, 4096, 4096, 4096, strides, 4096, 4, 4096, 1, 0, 1.0, 1, 65535, 1, 2, 0) == -2
+
+
+def test_rows_that_overlap_are_refused():
+    from morphserve_b200.worker.kernels.rotary_pos import _strides
+    base = torch.zeros(128)
+    for shape, stride in (((4, 3, 8), (8, 8, 1)), ((4, 3, 8), (16, 8, 1)), ((4, 3, 8), (8, 16, 1)), ((2, 2, 8), (15, 8, 1)),
+                          ((2, 1, 8), (7, 8, 1)), ((1, 2, 8), (8, 7, 1)), ((2, 2, 8), (16, 8, 2))):
+        with pytest.raises(AssertionError):
+            _strides(base.as_strided(shape, stride), shape[0], shape[1], shape[2])
+    for shape, stride in (((2, 3, 8), (24, 8, 1)), ((2, 3, 8), (8, 16, 1)), ((2, 2, 8), (17, 9, 1)), ((1, 3, 8), (0, 8, 1)),
+                          ((2, 1, 8), (8, 0, 1))):
+        assert _strides(base.as_strided(shape, stride), shape[0], shape[1], shape[2]) == stride
+
+
+def test_yarn_variants_are_refused(mk):
+    sc = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
+    for more in ({"mscale": 1.0}, {"mscale_all_dim": 0.5}, {"truncate": False}):
+        with pytest.raises(ValueError):
+            mk.rotary_inv_freq(cfg(rope_scaling={**sc, **more}), device="cpu")
+    assert mk.rotary_inv_freq(cfg(rope_scaling={**sc, "truncate": True, "mscale": None}), device="cpu")[1] > 1
