@@ -501,6 +501,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     float qfac[NT][2];      // scale_log2 and what undoes the normalisation of a bf16 q, for heads 2t and 2t + 1
     float kinit[NT][2];     // what takes the offset of int8 codes out of the scores
     float thr[NT][2], base[NT][2], l[NT][2];
+    constexpr bool kRest = !DUP;    // what fp16 leaves over of the weights goes through products of its own
+    float rest_off[NT][4];          // int8: -128 times the sum of those, which all dims share, until the piece ends
     bool piece_starts = false;
     // byte offsets inside a half: K pieces of tokens g and g + 8; V rows and pieces for ldmatrix
     const uint32_t k_at = D == 128 ? g * 128 + (((2 * t) ^ g) << 4) : (g >> 1) * 128 + ((((g & 1) * 4 + t) ^ (g >> 1)) << 4);
@@ -584,6 +586,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+                rest_off[n][0] = rest_off[n][1] = rest_off[n][2] = rest_off[n][3] = 0.f;
                 thr[n][0] = thr[n][1] = -INFINITY;
                 base[n][0] = base[n][1] = l[n][0] = l[n][1] = 0.f;
             }
@@ -654,9 +657,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                             o[n][i][e] *= a;
                             o[n][i][e + 2] *= a;
                         }
+                        rest_off[n][e] *= a;
+                        rest_off[n][e + 2] *= a;
                     }
             }
-            uint32_t pb[NT][2];
+            uint32_t pb[NT][2], pr[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float w0 = ex2(sc[n][0] - base[n][0]), w1 = ex2(sc[n][1] - base[n][1]);
@@ -664,11 +669,14 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 l[n][0] = fmaf(w0 + w2, iv, l[n][0]);
                 l[n][1] = fmaf(w1 + w3, iv, l[n][1]);
                 __half2 x = __floats2half2_rn(w0, w1), y = __floats2half2_rn(w2, w3);
+                const float2 fx = __half22float2(x), fy = __half22float2(y);
+                const __half2 rx = __floats2half2_rn(w0 - fx.x, w1 - fx.y), ry = __floats2half2_rn(w2 - fy.x, w3 - fy.y);
                 if (DUP) {  // columns 4-7: what the rounding of columns 0-3 left over
-                    const float2 fx = __half22float2(x), fy = __half22float2(y);
-                    const __half2 rx = __floats2half2_rn(w0 - fx.x, w1 - fx.y), ry = __floats2half2_rn(w2 - fy.x, w3 - fy.y);
                     x = t >= 2 ? rx : x;
                     y = t >= 2 ? ry : y;
+                } else {    // ... of all columns: a second B operand
+                    pr[n][0] = transpose8x8(half2_bits(rx));
+                    pr[n][1] = transpose8x8(half2_bits(ry));
                 }
                 pb[n][0] = transpose8x8(half2_bits(x));
                 pb[n][1] = transpose8x8(half2_bits(y));
@@ -682,6 +690,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
                         mma(o[n][c], kMinusOffset2, kMinusOffset2, kMinusOffset2, kMinusOffset2, pb[n][0], pb[n][1]);
+                if (kRest) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        mma(rest_off[n], kMinusOffset2, kMinusOffset2, kMinusOffset2, kMinusOffset2, pr[n][0], pr[n][1]);
+                }
             }
 #pragma unroll
             for (int c = 0; c < MT; c += 2) {
@@ -692,13 +705,19 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     const uint32_t lo = n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u, hi = n >= 10 ? 0xffffffffu : n == 9 ? 0xffffu : 0u;
                     w[0] &= lo; w[1] &= hi; w[2] &= lo; w[3] &= hi;
                 }
+                uint32_t a[2][4];
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    uint32_t a0, a1, a2, a3;
-                    widen_v<CODE>(w[2 * d], masks, a0, a1);
-                    widen_v<CODE>(w[2 * d + 1], masks, a2, a3);
+                    widen_v<CODE>(w[2 * d], masks, a[d][0], a[d][1]);
+                    widen_v<CODE>(w[2 * d + 1], masks, a[d][2], a[d][3]);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma(o[n][c + d], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                    for (int n = 0; n < NT; ++n) mma(o[n][c + d], a[d][0], a[d][1], a[d][2], a[d][3], pb[n][0], pb[n][1]);
+                }
+                if (kRest) {
+#pragma unroll
+                    for (int d = 0; d < 2; ++d)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma(o[n][c + d], a[d][0], a[d][1], a[d][2], a[d][3], pr[n][0], pr[n][1]);
                 }
             }
         }
@@ -721,6 +740,12 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[n][i][e] += __shfl_xor_sync(0xffffffffu, o[n][i][e], 2);
+                }
+                if (kRest && CODE == MKV_Q8_INT8) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][i][e] += rest_off[n][e];
                 }
             }
             float *row = nullptr;
@@ -941,7 +966,11 @@ constexpr int kBlocksPerSm = 1;
 constexpr size_t kErrorBytes = 256;     // error word, then the arrival counters
 
 static size_t zero_bytes(int sms) { return kErrorBytes + (((size_t)sms * kBlocksPerSm * sizeof(int) + 255) & ~(size_t)255); }
-// Query heads of a unit: 4 (columns 4-7 of the tile then carry what fp16 loses of the weights), 8 or 16.
+// Query heads of a unit: 4, 8 or 16.  The weights enter the second product as an fp16 number and what that leaves over, also
+// fp16 (2^-22 of the weight together).  With 4 heads the remainders are columns 4-7 of the tile and cost nothing; with 8 and 16
+// they are a second B operand, twice the products of V: long contexts in groups of 8, e4m3 68.7 -> 73 us, int8 72 -> 80; 256
+// sequences in groups of 8 48.7 -> 53.5, of 16 65 -> 71.  Without them an output is off by 1.4e-4 of the weighted values' size,
+// which shows beside fp16's own rounding and is far above it where values cancel.
 static int unit_heads(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 
 static bool fast_shape(const PoolViewQ8 &pv) {

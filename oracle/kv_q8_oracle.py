@@ -142,28 +142,57 @@ def cached(segs, code, table, row, n, layer, bs):
     return (np.stack(ks), np.stack(vs), missing) if ks else (None, None, missing)
 
 
-def attention(segs, code, q, table, ids, lens, layer, bs, scale):
+def attention(segs, code, q, table, ids, lens, layer, bs, scale, weights=16):
     """(o, slack) [batch, q_heads, dim] float64; NaN rows where nothing is attended.  `slack` bounds what a kernel may be
     off before its output is rounded: weights rounded to fp16 (2^-11 of each, 2^-25 at least), scores summed in fp32 and
-    exponentials good to 2^-20."""
+    exponentials good to 2^-20.
+
+    `weights` = 32: what a kernel may be off that holds its weights to 32 bits or as an fp16 number and what that leaves
+    over (see slack_32)."""
     B, Hq, D = q.shape
     o, slack = np.full((B, Hq, D), np.nan), np.zeros((B, Hq, D))
     for i, n in enumerate(lens):
         if n <= 0:
             continue
-        k, v, _ = cached(segs, code, table, ids[i], n, layer, bs)
+        k, v, missing = cached(segs, code, table, ids[i], n, layer, bs)
         if k is None:
             continue
         G = Hq // k.shape[1]
+        if weights == 32:
+            at = [page(segs, table, ids[i], t // bs) for t in range(n) if t not in set(missing)]
+            sk, sv = (np.stack([seg[c][r, layer] for seg, r in at]).astype(np.float64) for c in ("ks", "vs"))
         for h in range(Hq):
             x, kk, vv = q[i, h].astype(np.float64), k[:, h // G], v[:, h // G]
             s = kk @ x * scale
             p = np.exp(s - s.max())
             total = p.sum()
             o[i, h] = p @ vv / total
+            if weights == 32:
+                slack[i, h] = slack_32(code, x, kk, vv, sk[:, h // G], sv[:, h // G], p, scale)
+                continue
             off = (D + 8) * 2.0 ** -24 * (np.abs(kk) @ np.abs(x)).max() * abs(scale)
             slack[i, h] = (2.0 ** -11 + 2 * off + 2.0 ** -20) * (p @ np.abs(vv)) / total + len(p) * 2.0 ** -25 * np.abs(vv).max(0) / total
     return o, slack
+
+
+def slack_32(code, x, k, v, sk, sv, p, scale):
+    """What one row of the attention may be off with weights to 32 bits; sk, sv: the tokens' scales, p: their weights.
+
+    Scores: a product for each element of x that is not 0 and a few more roundings, 2^-23 each (a tensor core cuts off
+    where an adder rounds), of the sum of absolute values - with int8 codes held as q + 128, whose 128 is taken off again,
+    of up to 255 s |x|.  log2 of V's scale joins the exponent: good to 2^-22 of itself, and the sum rounds once more.
+    A weight: exponential 2^-22, its fp16 number's remainder as fp16 2^-22, 2^-31 of the largest at least (fp16's smallest
+    half step 2^-25, with the largest weight held at 2^6 or more).
+    Sums over tokens: up to three products for 16 tokens, a piece's merge, or one addition a token: 2^-23 each, of the sum
+    of absolute values, with int8 codes again up to 255 s."""
+    total, n = p.sum(), len(p)
+    size = 255 * sk[:, None] if code == "int8" else np.abs(k)
+    off = (np.count_nonzero(x) + 8) * 2.0 ** -23 * (size * np.abs(x)).sum(1).max() * abs(scale)
+    log_sv = np.abs(np.log2(np.maximum(sv, TINY))).max()
+    rel = 2 * off + (log_sv + 4) * 2.0 ** -22
+    mass = p @ (255 * sv[:, None] * np.ones_like(v) if code == "int8" else np.abs(v))
+    steps = 3 * -(-n // 16) + n + 16
+    return (rel * (p @ np.abs(v)) + steps * 2.0 ** -23 * mass + n * 2.0 ** -31 * (p * sv).max() * 448) / total
 
 
 def rotary(x, positions, inv_freq, interleaved, attention_scale):

@@ -1,0 +1,64 @@
+"""GPU: how many bits the attention over the 8-bit pool keeps.  Outputs that nearly cancel are small beside the weighted
+values they are the sum of, so that the output's own rounding does not hide what the weights lost."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_q8_oracle as O
+
+from .test_gpu_kv_q8 import CODES, DTYPES, HALF, Case, mk  # noqa: F401  (mk: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def cancelling(code, lens, hq, hkv, d, bs, seed):
+    """A case and its queries: head h of a group asks for one element of K alone, and in the dims d = h (mod group) V has two
+    tokens, whose codes are chosen so that their weighted sum is close to 0 there; the other tokens' values are 0."""
+    c = Case(code, lens, hq=hq, hkv=hkv, d=d, bs=bs, seed=seed)
+    group = hq // hkv
+    table = O.INT8 if code == "int8" else O.E4M3
+    q = np.zeros((len(lens), hq, d))
+    for h in range(hq):
+        q[:, h, h % group] = 2.0 ** c.rs.randint(1, 4, len(lens))
+    big = np.array([x for x in range(256) if np.isfinite(table[x]) and 30 <= abs(table[x]) <= 127])
+    for i, n in enumerate(lens):
+        k, _, _ = O.cached(c.segs, code, c.table, c.ids[i], n, c.layer, bs)
+        at = [O.page(c.segs, c.table, c.ids[i], t // bs) for t in range(n)]
+        for t in range(n):
+            at[t][0]["v"][at[t][1], c.layer, :, t % bs] = 0
+        for hk in range(hkv):
+            for e in range(d):
+                h = hk * group + e % group
+                s = k[:, hk] @ q[i, h] * c.scale
+                a, b = 0, n - 1
+                w = [np.exp(s[t] - s[b]) * at[t][0]["vs"][at[t][1], c.layer, hk] for t in (a, b)]
+                one = c.rs.choice(big, 24)
+                want = -table[one] * w[0] / w[1]
+                best = np.abs(table[big][None] - want[:, None])
+                pick = np.unravel_index(np.argmin(best / np.abs(want)[:, None]), best.shape)
+                at[a][0]["v"][at[a][1], c.layer, hk, a % bs, e] = one[pick[0]]
+                at[b][0]["v"][at[b][1], c.layer, hk, b % bs, e] = big[pick[1]]
+    for g, s in zip(c.gpu, c.segs):
+        g["v"].copy_(c._codes(s["v"]))
+    return c, q
+
+
+# groups of 1 ... 20 query heads (units of 4, 8 and 16), both dims of the tensor-core kernel, and shapes of the plain one
+SHAPES = [(2, 2, 128, 16), (8, 2, 128, 16), (8, 2, 64, 16), (5, 1, 128, 16), (16, 2, 128, 16), (8, 1, 64, 32), (16, 1, 128, 16),
+          (20, 1, 128, 16), (24, 2, 64, 16), (8, 1, 80, 16), (4, 1, 128, 8)]
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hq,hkv,d,bs", SHAPES)
+def test_attention_keeps_its_weights_to_32_bits(mk, code, dtype, hq, hkv, d, bs):  # noqa: F811
+    lens = [2, 2, 2, 17, 33, 40]
+    c, qn = cancelling(code, lens, hq, hkv, d, bs, seed=hq * 100 + d)
+    t = DTYPES[dtype]
+    q = torch.from_numpy(qn).to(t).cuda()
+    got = c.attend(mk, q, c.state()).double().cpu().numpy().reshape(qn.shape)
+    want, slack = O.attention(c.segs, code, qn, c.table, c.ids, lens, c.layer, bs, c.scale, weights=32)
+    half, least = HALF[t]
+    room = half * np.abs(want) * (1 + 2.0 ** -6) + slack + least
+    off = np.abs(got - want)
+    assert (off <= room).all(), f"{(off / room).max():.3g} of the room"
