@@ -156,14 +156,14 @@ __device__ __forceinline__ bool named_again(const StoreQ8Args &a, int i, int row
 // as one contiguous tile.  NV = 0: pages that do not fit are read twice.
 // HBM bound: 64 prompts of up to 1536 tokens, 8 heads of 128 fp16, 54 us = 5.8 TB/s read and written (copy peak 6.55).
 template <typename T, int CODE, int V, int NV>
-__device__ __forceinline__ float store_tile(const StoreQ8Args &a, const T *src, int stride, uint8_t *dst, int total, int vecs, int lane) {
+__device__ __forceinline__ float store_tile(const StoreQ8Args &a, const T *src, int64_t stride, uint8_t *dst, int total, int vecs, int lane) {
     uint32_t peak = 0;
     if constexpr (NV > 0) {
         Piece<T, V> x[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int e = min(lane + 32 * j, total - 1), tok = (int)__umulhi((uint32_t)e, a.vecs_magic);  // behind the end: the last one again
-            x[j].load(src + tok * stride + (e - tok * vecs) * V);
+            x[j].load(src + tok * (int)stride + (e - tok * vecs) * V);  // (wide_ok: a page's rows are counted in 32 bits)
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) peak = x[j].peak(peak);
@@ -175,12 +175,12 @@ __device__ __forceinline__ float store_tile(const StoreQ8Args &a, const T *src, 
     } else {
         Piece<T, V> x;
         for (int e = lane; e < total; e += 32) {
-            x.load(src + (int64_t)(e / vecs) * stride + (e % vecs) * V);
+            x.load(src + (e / vecs) * stride + (e % vecs) * V);
             peak = x.peak(peak);
         }
         const float s = scale_of<CODE>(__reduce_max_sync(0xffffffffu, Piece<T, V>::peak_bits(peak))), inv = inverse_of(s);
         for (int e = lane; e < total; e += 32) {
-            x.load(src + (int64_t)(e / vecs) * stride + (e % vecs) * V);
+            x.load(src + (e / vecs) * stride + (e % vecs) * V);
             x.template store_codes<CODE>(dst + (int64_t)e * V, inv);
         }
         return s;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kHeadWarps * 32, sizeof(T) == 4 ? 2 : 4) store
                     const int64_t stride = which ? a.v_stride : a.k_stride;
                     const T *src = (const T *)(which ? a.v : a.k) + (start + lb * bs) * stride + (int64_t)h * D;
                     uint8_t *dst = (which ? a.pool.v_base[seg] : a.pool.k_base[seg]) + tile * a.pool.tile_bytes;
-                    const float s = store_tile<T, CODE, V, NV>(a, src, (int)stride, dst, total, vecs, lane);
+                    const float s = store_tile<T, CODE, V, NV>(a, src, stride, dst, total, vecs, lane);
                     if (lane == 0) (which ? a.pool.v_scale[seg] : a.pool.k_scale[seg])[tile] = s;
                 }
             }
