@@ -197,13 +197,13 @@ __global__ void __launch_bounds__(kHeadWarps * 32, sizeof(T) == 4 ? 2 : 4) store
         const int len = (int)min((int64_t)a.seq_lens[i], start < 0 ? 0 : a.num_tokens - start);
         if ((int64_t)blockIdx.x * bs >= len) continue;
         bool again = false;
-        for (int lb = blockIdx.x; (int64_t)lb * bs < len; lb += gridDim.x) {
+        for (int64_t lb = blockIdx.x; lb * bs < len; lb += gridDim.x) {     // (64 bits: a step may end behind what 32 count)
             int seg = 0;
-            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, lb, a.cur_layer, seg);
-            if (lb == (int)blockIdx.x) again = named_again(a, i, row);
+            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, (int)lb, a.cur_layer, seg);
+            if (lb == blockIdx.x) again = named_again(a, i, row);
             if (again) break;
             if (tile0 < 0) continue;
-            const int total = min(bs, len - lb * bs) * vecs;
+            const int total = min(bs, (int)(len - lb * bs)) * vecs;
             for (int h = blockIdx.z * warps + warp; h < Hkv; h += gridDim.z * warps) {
                 const int64_t tile = tile0 + h;
 #pragma unroll 1
@@ -308,12 +308,12 @@ __global__ void __launch_bounds__(kLoadThreads, 4) load_q8_kernel(const __grid_c
         const int64_t end = min((int64_t)a.ends[i], a.num_out_rows - shift);
         const int64_t begin = max((int64_t)max(first_tok, 0), -shift);   // (a negative start_locs entry reaches no row in front of the output)
         if (begin >= end) continue;
-        for (int lb = (int)begin / bs + blockIdx.x; (int64_t)lb * bs < end; lb += gridDim.x) {
+        for (int64_t lb = (int)begin / bs + (int64_t)blockIdx.x; lb * bs < end; lb += gridDim.x) {
             int seg = 0;
-            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, lb, a.cur_layer, seg);
+            const int64_t tile0 = page_of(a.pool, a.block_table, a.table_cols, a.num_rows, row, (int)lb, a.cur_layer, seg);
             if (tile0 < 0) continue;
-            const int first = max((int)begin, lb * bs);
-            const int total = ((int)min(end, ((int64_t)lb + 1) * bs) - first) * vecs, chunks = (total + 31) / 32, all = chunks * 2 * Hkv;
+            const int first = max((int)begin, (int)(lb * bs));
+            const int total = ((int)min(end, (lb + 1) * bs) - first) * vecs, chunks = (total + 31) / 32, all = chunks * 2 * Hkv;
             const int tile_bytes = (int)a.pool.tile_bytes, skip = (int)(first - lb * bs) * D, step = gridDim.z * (kLoadThreads / 32);
             for (int c0 = blockIdx.z * (kLoadThreads / 32) + warp; c0 < all; c0 += kLoadFlight * step) {
                 if constexpr (V == 16) {
@@ -421,8 +421,8 @@ int mkv_store_kv_q8_prefill(int device, void *stream, const void *k, const void 
     a.seq_ids = seq_ids; a.start_locs = start_locs; a.seq_lens = seq_lens; a.num_seqs = num_seqs; a.cur_layer = cur_layer;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return set_cuda_error(guard.err);
-    const dim3 grid((unsigned)ceil_div64(max_seq_len, a.pool.block_size), (unsigned)std::min(num_seqs, 65535),
-                    blocks_for(a.pool.num_kv_heads, kHeadWarps));
+    const dim3 grid((unsigned)std::min(ceil_div64(max_seq_len, a.pool.block_size), table_stride), (unsigned)std::min(num_seqs, 65535),
+                    blocks_for(a.pool.num_kv_heads, kHeadWarps));   // (no page stands behind the table's last column)
     const int threads = warps_for(a.pool.num_kv_heads, kHeadWarps) * 32;
     a.vecs_magic = magic_of(a.pool.head_dim / 16);
     const int64_t pieces = a.pool.tile_bytes / 16;
@@ -495,7 +495,7 @@ int mkv_load_kv_q8(int device, void *stream, void *k, void *v, int64_t k_stride,
     const int64_t pages = num_out_rows / a.pool.block_size + 2 * (int64_t)num_seqs;
     const int64_t chunks = ceil_div64(a.pool.tile_bytes / (wide ? 16 : 1), 32) * 2 * a.pool.num_kv_heads;
     const int64_t rounds = num_out_rows >= (int64_t)num_seqs * a.pool.block_size && chunks * pages >= 8 * (kLoadThreads / 32) * 4ll * sms ? 8 : 4;
-    const dim3 grid((unsigned)(ceil_div64(max_len, a.pool.block_size) + 1), (unsigned)std::min(num_seqs, 65535),
+    const dim3 grid((unsigned)std::min(ceil_div64(max_len, a.pool.block_size) + 1, table_stride), (unsigned)std::min(num_seqs, 65535),
                     (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks / (rounds * (kLoadThreads / 32)), 65535)));
     dispatch(dtype, a.pool.code, wide, [&](auto t, auto code, auto w) {
         load_q8_kernel<decltype(t), decltype(code)::value, decltype(w)::value>

@@ -33,3 +33,20 @@ def test_rows_further_apart_than_32_bits_count(mk, code, apart):  # noqa: F811
     mk.load_kvcache_q8(k, v, *c.pool(), c.table_t, c.mc, c.ec, i32(c.ids[:1]), i32([0]), i32([3]), i32([0]), 3, c.layer)
     for got, want in zip((k, v), O.cached(c.segs, code, c.table, c.ids[0], 3, c.layer, c.bs)):
         assert (np.abs(got.double().cpu().numpy() - want) <= (2.0 ** -11 + 2.0 ** -23) * np.abs(want) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("bs", [1, 16])
+def test_a_length_hint_far_above_the_lengths(mk, bs):  # noqa: F811
+    """max_prefill_len and max_len size a launch only: the largest 32-bit number does no more than the lengths themselves."""
+    c = Case("int8", [7, 20], hkv=2, d=32, bs=bs, seed=41)
+    k, kn = c.rows(27, 2, torch.float16)
+    v, vn = c.rows(27, 2, torch.float16)
+    st = c.state(prefill=[7, 20], decode=[])
+    st.max_prefill_len = 2 ** 31 - 1
+    mk.store_kvcache_q8(k, v, *c.pool(), c.table_t, c.mc, c.ec, st, c.layer)
+    O.store_prefill(c.segs, "int8", kn, vn, c.table, c.ids, [0, 7], [7, 20], c.layer, bs)
+    c.same()
+    mk.load_kvcache_q8(k, v, *c.pool(), c.table_t, c.mc, c.ec, i32(c.ids), i32([0, 3]), i32([7, 20]), i32([0, 7]), 2 ** 31 - 1, c.layer)
+    want = [np.concatenate([a, b[3:]]) for a, b in zip(*(O.cached(c.segs, "int8", c.table, i, n, c.layer, bs)[:2] for i, n in zip(c.ids, (7, 20))))]
+    for got, w in zip((k, v), want):
+        assert (np.abs(got[:24].double().cpu().numpy() - w) <= (2.0 ** -11 + 2.0 ** -23) * np.abs(w) + 2.0 ** -25).all()
