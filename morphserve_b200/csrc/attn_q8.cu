@@ -32,9 +32,19 @@
 namespace mkv {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLargest = 3.402823466e38f;     // of fp32
+
+// The smaller one; NaN if either is NaN.
+__device__ __forceinline__ float min_nan(float x, float y) {
+    float z;
+    asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
 
 // ------------------------------------------------------------------ plain kernel
-// One warp per (sequence, query head); lane l holds dims l, l + 32, ...  fp32 throughout.
+// One warp per (sequence, query head); lane l holds dims l, l + 32, ...  fp32 throughout.  Weights are held as unit * 2^(score -
+// max), whose sum l stays below 5/8: so the weighted sum of values is no larger than the largest of them.  Likewise a power of two
+// takes the query's largest element to [1, 2), so that its products with codes are ordinary numbers whatever the score is made of.
 constexpr int kPlainDims = 16;  // head_dim <= 512
 
 template <typename T, int CODE>
@@ -58,7 +68,14 @@ __global__ void attn_q8_plain_kernel(const T *__restrict__ q, int64_t q_stride, 
         qr[i] = d < D ? value_of<T>(q[b * q_stride + (int64_t)hq * D + d]) : 0.f;
         acc[i] = 0.f;
     }
-    float m = -INFINITY, l = 0.f;
+    uint32_t peak = 0;
+#pragma unroll
+    for (int i = 0; i < kPlainDims; ++i) peak = max(peak, __float_as_uint(qr[i]) & 0x7fffffffu);
+    const int e = min(max((int)(__reduce_max_sync(0xffffffffu, peak) >> 23), 1), 253);
+    const float up = __uint_as_float((uint32_t)e << 23), down = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < kPlainDims; ++i) qr[i] *= down;
+    float m = -INFINITY, l = 0.f, unit = 0.125f;
     bool bad = row < 0 || row >= num_rows;
     const int nblk = bad ? 0 : (int)min(((int64_t)len + bs - 1) / bs, table_stride);
     bad |= (int64_t)nblk * bs < len;
@@ -73,7 +90,8 @@ __global__ void attn_q8_plain_kernel(const T *__restrict__ q, int64_t q_stride, 
         locate_block(pool, blk, seg, brow);
         const int64_t tile = tile_index(pool, brow, cur_layer, h);
         const uint8_t *kt = pool.k_base[seg] + tile * pool.tile_bytes, *vt = pool.v_base[seg] + tile * pool.tile_bytes;
-        const float ks = pool.k_scale[seg][tile] * scale_log2, vs = pool.v_scale[seg][tile];
+        // (a factor too large for 32 bits: 0 times it is 0 all the same)
+        const float ks = min_nan(pool.k_scale[seg][tile] * up * scale_log2, kLargest), vs = pool.v_scale[seg][tile];
         const int ntok = (int)min((int64_t)bs, len - (int64_t)jb * bs);
         for (int tk = 0; tk < ntok; ++tk) {
             float dot = 0.f;
@@ -86,7 +104,12 @@ __global__ void attn_q8_plain_kernel(const T *__restrict__ q, int64_t q_stride, 
             for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
             const float sc = dot * ks;
             const float mn = fmaxf(m, sc), base = mn == -INFINITY ? 0.f : mn;  // no finite score yet: all weights are 0
-            const float a = exp2f(m - base), w = exp2f(sc - base);
+            float a = exp2f(m - base);
+            if (l * a > 0.5f) {
+                a *= 0.5f;
+                unit *= 0.5f;
+            }
+            const float w = exp2f(sc - base) * unit;
             l = l * a + w;
 #pragma unroll
             for (int i = 0; i < kPlainDims; ++i) {

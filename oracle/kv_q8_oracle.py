@@ -182,14 +182,16 @@ def slack_32(code, x, k, v, sk, sv, p, scale):
     where an adder rounds), of the sum of absolute values - with int8 codes held as q + 128, whose 128 is taken off again,
     of up to 255 s |x|.  log2 of V's scale joins the exponent: good to 2^-22 of itself, and the sum rounds once more.
     A weight: exponential 2^-22, its fp16 number's remainder as fp16 2^-22, 2^-31 of the largest at least (fp16's smallest
-    half step 2^-25, with the largest weight held at 2^6 or more).
+    half step 2^-25, with the largest weight held at 2^6 or more).  The denominator's factor and the output's two take
+    2^-22 each, and as much is left for the factors by which a maximum that moves scales sums down (2 * 2^-22 on what then
+    has 2^-4 of the weight or less).
     Sums over tokens: up to three products for 16 tokens, a piece's merge, or one addition a token: 2^-23 each, of the sum
     of absolute values, with int8 codes again up to 255 s."""
     total, n = p.sum(), len(p)
     size = 255 * sk[:, None] if code == "int8" else np.abs(k)
     off = (np.count_nonzero(x) + 8) * 2.0 ** -23 * (size * np.abs(x)).sum(1).max() * abs(scale)
-    log_sv = np.abs(np.log2(np.maximum(sv, TINY))).max()
-    rel = 2 * off + (log_sv + 4) * 2.0 ** -22
+    log_sv = np.abs(np.log2(sv, out=np.zeros_like(sv), where=sv > 0)).max()
+    rel = 2 * off + (1.25 * log_sv + 6) * 2.0 ** -22
     mass = p @ (255 * sv[:, None] * np.ones_like(v) if code == "int8" else np.abs(v))
     steps = 3 * -(-n // 16) + n + 16
     return (rel * (p @ np.abs(v)) + steps * 2.0 ** -23 * mass + n * 2.0 ** -31 * (p * sv).max() * 448) / total

@@ -62,3 +62,51 @@ def test_attention_keeps_its_weights_to_32_bits(mk, code, dtype, hq, hkv, d, bs)
     room = half * np.abs(want) * (1 + 2.0 ** -6) + slack + least
     off = np.abs(got - want)
     assert (off <= room).all(), f"{(off / room).max():.3g} of the room"
+
+
+def check_32(c, o, qn):
+    want, slack = O.attention(c.segs, c.code, qn, c.table, c.ids, c.lens, c.layer, c.bs, c.scale, weights=32)
+    half, least = HALF[o.dtype]
+    got = o.double().cpu().numpy().reshape(want.shape)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), f"NaN in {np.argwhere(np.isnan(got) != np.isnan(want))[:4].tolist()}"
+    room = half * np.abs(want) * (1 + 2.0 ** -6) + slack + least
+    off = np.abs(got - want)
+    assert (off <= room).all(), f"{np.nanmax(off / room):.3g} of the room at {np.argwhere(off > room)[:4].tolist()}"
+
+
+def scales(c, name, exponents):
+    """Scales 2^exponent (int8: up to twice that) in place of the case's, one for each block and head."""
+    for g, s in zip(c.gpu, c.segs):
+        x = 2.0 ** c.rs.choice(exponents, s[name].shape)
+        s[name][:] = (x * c.rs.uniform(1, 2, x.shape) if c.code == "int8" else x).astype(np.float32)
+        g[name].copy_(c._dev(s[name]))
+
+
+# shapes of the plain kernel
+PLAIN = [(4, 2, 80)]
+EXTREME_LENS = [1, 16, 17, 40, 100, 333, 64]
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hq,hkv,d", PLAIN)
+@pytest.mark.parametrize("exponents", [range(-126, -109), range(108, 119), range(-40, 11), range(-126, 119), [-126, 118]],
+                         ids=["tiny", "huge", "spread", "all", "both ends"])
+def test_attention_takes_every_scale_of_v(mk, code, hq, hkv, d, exponents):  # noqa: F811
+    """Scales that a cache of bf16 rows can have, down to the smallest normal number and up to the largest."""
+    c = Case(code, EXTREME_LENS, hq=hq, hkv=hkv, d=d, seed=d + hq)
+    scales(c, "vs", list(exponents))
+    q, qn = c.rows(len(c.lens), hq, torch.bfloat16)
+    check_32(c, c.attend(mk, q, c.state()), qn)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hq,hkv,d", PLAIN)
+@pytest.mark.parametrize("exponent", [-126, -100, 100, 106, 118])
+def test_attention_takes_every_scale_of_k(mk, code, hq, hkv, d, exponent):  # noqa: F811
+    """... with queries that bring the scores back to ordinary sizes, or are 0."""
+    c = Case(code, EXTREME_LENS, hq=hq, hkv=hkv, d=d, seed=d + hq + 1)
+    scales(c, "ks", [exponent, exponent - 1 if exponent > 0 else exponent + 1])
+    q, _ = c.rows(len(c.lens), hq, torch.float32)
+    q = (q * 2.0 ** (-exponent // 2) * 2.0 ** (-7 - exponent - (-exponent // 2))).to(torch.bfloat16)
+    q[1], q[4, 1], q[5, -1] = 0, 0, 0
+    check_32(c, c.attend(mk, q, c.state()), q.double().cpu().numpy())
