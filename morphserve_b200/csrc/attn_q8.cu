@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
         for (int h = 0; h < 2; ++h) {
             const uint32_t at = st + h * HB;
             const int tokens = (int)((ma.x >> (8 + 8 * h)) & 0xffu);
-            const float ks = __uint_as_float(h ? scales.y : scales.x) * (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f), vs = __uint_as_float(h ? scales.w : scales.z);
+            const float ks = __uint_as_float(h ? scales.y : scales.x), vs = __uint_as_float(h ? scales.w : scales.z);
             // ---- S^T = K Q^T
             float sc[NT][4];
 #pragma unroll
@@ -653,7 +653,10 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
             bool above = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float f0 = (kScaledQ ? qfac[n][0] : p.scale_log2) * ks, f1 = (kScaledQ ? qfac[n][1] : p.scale_log2) * ks;
+                // (a factor too large for 32 bits: 0 times it is 0 all the same)
+                constexpr float kUnit = CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f;
+                const float f0 = min_nan((kScaledQ ? qfac[n][0] : p.scale_log2) * ks * kUnit, kLargest);
+                const float f1 = kScaledQ ? min_nan(qfac[n][1] * ks * kUnit, kLargest) : f0;
                 sc[n][0] = on0 ? fmaf(sc[n][0], f0, lv) : -INFINITY;
                 sc[n][1] = on0 ? fmaf(sc[n][1], f1, lv) : -INFINITY;
                 sc[n][2] = on1 ? fmaf(sc[n][2], f0, lv) : -INFINITY;

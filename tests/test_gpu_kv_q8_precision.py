@@ -82,8 +82,9 @@ def scales(c, name, exponents):
         g[name].copy_(c._dev(s[name]))
 
 
-# shapes of the plain kernel
-PLAIN = [(4, 2, 80)]
+# groups of 2, 8 and 16 on the tensor cores in both dims, and the plain kernel
+EXTREME = [(4, 2, 128), (4, 2, 64), (8, 1, 128), (16, 1, 128), (16, 1, 64), (4, 2, 80)]
+PLAIN = EXTREME[-1:]
 EXTREME_LENS = [1, 16, 17, 40, 100, 333, 64]
 
 
@@ -100,7 +101,7 @@ def test_attention_takes_every_scale_of_v(mk, code, hq, hkv, d, exponents):  # n
 
 
 @pytest.mark.parametrize("code", CODES)
-@pytest.mark.parametrize("hq,hkv,d", PLAIN)
+@pytest.mark.parametrize("hq,hkv,d", EXTREME)
 @pytest.mark.parametrize("exponent", [-126, -100, 100, 106, 118])
 def test_attention_takes_every_scale_of_k(mk, code, hq, hkv, d, exponent):  # noqa: F811
     """... with queries that bring the scores back to ordinary sizes, or are 0."""
