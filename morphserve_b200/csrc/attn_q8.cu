@@ -134,7 +134,8 @@ constexpr int kUnitCost = 2;      // phantom tiles in front of a (sequence, head
                                   // us, the 64-sequence one 53.3, 52.2, 54.0, the long contexts 69.0, 69.2, 70.5
 constexpr float kBoost = 6.f;     // weights are held as 2^(score - max + 6): fp16 then reaches 2^-20 of the largest in full
 constexpr float kLag = 4.f;       // the running maximum follows only when a score is above it by 2^4
-constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
+constexpr float kFaint = 90.f;    // how far log2 of a V scale may lie below the reference before its weights are summed apart
+constexpr float kAhead = 64.f;    // ... whose scores may then be above theirs by as much
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint64_t policy) {
@@ -178,6 +179,12 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
+}
+// Over the lanes of a column of S^T.
+__device__ __forceinline__ float column_max(float m) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+    return fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
@@ -523,7 +530,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
     uint32_t qf[NT][KW][2];
     float qfac[NT][2];      // scale_log2 and what undoes the normalisation of a bf16 q, for heads 2t and 2t + 1
     float kinit[NT][2];     // what takes the offset of int8 codes out of the scores
-    float thr[NT][2], base[NT][2], l[NT][2];
+    float thr[NT][2], base[NT][2], l[NT][2], ref[NT][2];
     constexpr bool kRest = !DUP;    // what fp16 leaves over of the weights goes through products of its own
     float rest_off[NT][4];          // int8: -128 times the sum of those, which all dims share, until the piece ends
     bool piece_starts = false;
@@ -612,6 +619,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 rest_off[n][0] = rest_off[n][1] = rest_off[n][2] = rest_off[n][3] = 0.f;
                 thr[n][0] = thr[n][1] = -INFINITY;
                 base[n][0] = base[n][1] = l[n][0] = l[n][1] = 0.f;
+                ref[n][0] = ref[n][1] = INFINITY;
             }
         }
 
@@ -642,70 +650,96 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 }
             }
             // ---- softmax: token g (elements 0, 1) and g + 8 (2, 3), heads 2t, 2t + 1
-            // The block's V scale joins the exponent: weights are 2^(score + log2 s_v - base), so that O accumulates across
-            // blocks as the tensor core leaves it, and the denominator takes them back over s_v.  A scale below 2^-100 (an
-            // all-zero block's, above all) counts as 2^-100, and does not move the maximum.
-            const float sv = vs < kLeastScale ? kLeastScale : vs;
-            float lv, iv;
-            asm("lg2.approx.f32 %0, %1;\n" : "=f"(lv) : "f"(sv));
-            asm("rcp.approx.f32 %0, %1;\n" : "=f"(iv) : "f"(sv));
+            // The block's V scale joins the exponent: weights are w = 2^(score + log2 s_v - base), so that O accumulates across
+            // blocks as the tensor core leaves it.  The denominator l takes 2^ref / s_v of them, that is 2^(score - (base - ref)):
+            // ref is log2 s_v of the half that moved base last, or less, so that base - ref, about that half's largest score, never
+            // falls and l never grows when base moves.  So all scales that fp32 holds are equally good.  Where s_v is below 2^ref
+            // by more than 2^90 (an all-zero block's, above all) w may be nothing although l needs it: then l takes the scores.
+            float lv;
+            asm("lg2.approx.f32 %0, %1;\n" : "=f"(lv) : "f"(vs));
             const bool on0 = g < tokens, on1 = g + 8 < tokens;
-            bool above = false;
+            bool above = false, apart[NT][2];      // apart: l has this half's weights already
+            float x[NT][4], fs[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+                apart[n][0] = apart[n][1] = false;
                 // (a factor too large for 32 bits: 0 times it is 0 all the same)
                 constexpr float kUnit = CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f;
-                const float f0 = min_nan((kScaledQ ? qfac[n][0] : p.scale_log2) * ks * kUnit, kLargest);
-                const float f1 = kScaledQ ? min_nan(qfac[n][1] * ks * kUnit, kLargest) : f0;
-                sc[n][0] = on0 ? fmaf(sc[n][0], f0, lv) : -INFINITY;
-                sc[n][1] = on0 ? fmaf(sc[n][1], f1, lv) : -INFINITY;
-                sc[n][2] = on1 ? fmaf(sc[n][2], f0, lv) : -INFINITY;
-                sc[n][3] = on1 ? fmaf(sc[n][3], f1, lv) : -INFINITY;
-                above |= fmaxf(sc[n][0], sc[n][2]) > thr[n][0] || fmaxf(sc[n][1], sc[n][3]) > thr[n][1];
+                fs[n][0] = min_nan((kScaledQ ? qfac[n][0] : p.scale_log2) * ks * kUnit, kLargest);
+                fs[n][1] = kScaledQ ? min_nan(qfac[n][1] * ks * kUnit, kLargest) : fs[n][0];
+                x[n][0] = on0 ? fmaf(sc[n][0], fs[n][0], lv) : -INFINITY;
+                x[n][1] = on0 ? fmaf(sc[n][1], fs[n][1], lv) : -INFINITY;
+                x[n][2] = on1 ? fmaf(sc[n][2], fs[n][0], lv) : -INFINITY;
+                x[n][3] = on1 ? fmaf(sc[n][3], fs[n][1], lv) : -INFINITY;
+                above |= fmaxf(x[n][0], x[n][2]) > thr[n][0] || fmaxf(x[n][1], x[n][3]) > thr[n][1];
+                above |= lv + kFaint < ref[n][0] || lv + kFaint < ref[n][1];
             }
             if (__any_sync(0xffffffffu, above)) {   // the maxima settle after the first tiles of a piece
+                bool faint = vs == 0.f;
+                if (!faint) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float m = fmaxf(sc[n][e], sc[n][e + 2]);
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                        m = fmaxf(m, thr[n][e] - kLag);
-                        const float to = m == -INFINITY ? 0.f : m - kBoost;
-                        const float a = thr[n][e] == -INFINITY ? 1.f : ex2(base[n][e] - to);   // before: all weights were 0
-                        thr[n][e] = m + kLag;
-                        base[n][e] = to;
-                        l[n][e] *= a;
+                        for (int e = 0; e < 2; ++e) {
+                            // a head moves by 2^4 at least, so that what its factors are off counts for tokens of small weight only
+                            const float m = column_max(fmaxf(x[n][e], x[n][e + 2]));
+                            const bool moves = m > thr[n][e];
+                            const float by = moves ? base[n][e] - (m - kBoost) : 0.f;
+                            const float a = thr[n][e] == -INFINITY ? 1.f : ex2(by);     // before: all weights were 0
+                            if (moves) {
+                                const float r = fminf(lv, ref[n][e] - by);
+                                l[n][e] *= ex2(by + (r - ref[n][e]));
+                                thr[n][e] = m + kLag;
+                                base[n][e] = m - kBoost;
+                                ref[n][e] = r;
+                            }
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            o[n][i][e] *= a;
-                            o[n][i][e + 2] *= a;
+                            for (int i = 0; i < MT; ++i) {
+                                o[n][i][e] *= a;
+                                o[n][i][e + 2] *= a;
+                            }
+                            rest_off[n][e] *= a;
+                            rest_off[n][e + 2] *= a;
+                            apart[n][e] = lv + kFaint < ref[n][e];
+                            faint |= apart[n][e];
                         }
-                        rest_off[n][e] *= a;
-                        rest_off[n][e + 2] *= a;
-                    }
+                }
+                if (__any_sync(0xffffffffu, faint)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float s0 = on0 ? sc[n][e] * fs[n][e] : -INFINITY, s1 = on1 ? sc[n][e + 2] * fs[n][e] : -INFINITY;
+                            const float m = column_max(fmaxf(s0, s1)), held = base[n][e] - ref[n][e];
+                            const float to = m > held + kAhead ? m : held;
+                            if ((apart[n][e] || vs == 0.f) && to > -INFINITY) {
+                                l[n][e] = l[n][e] * ex2(held - to) + (ex2(s0 - to) + ex2(s1 - to));
+                                ref[n][e] = base[n][e] - to;
+                            }
+                            if (isnan(s0 + s1)) l[n][e] = s0 + s1;
+                        }
+                    if (vs == 0.f) continue;    // (the same for the whole warp)
+                }
             }
             uint32_t pb[NT][2], pr[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float w0 = ex2(sc[n][0] - base[n][0]), w1 = ex2(sc[n][1] - base[n][1]);
-                const float w2 = ex2(sc[n][2] - base[n][0]), w3 = ex2(sc[n][3] - base[n][1]);
-                l[n][0] = fmaf(w0 + w2, iv, l[n][0]);
-                l[n][1] = fmaf(w1 + w3, iv, l[n][1]);
-                __half2 x = __floats2half2_rn(w0, w1), y = __floats2half2_rn(w2, w3);
-                const float2 fx = __half22float2(x), fy = __half22float2(y);
+                const float w0 = ex2(x[n][0] - base[n][0]), w1 = ex2(x[n][1] - base[n][1]);
+                const float w2 = ex2(x[n][2] - base[n][0]), w3 = ex2(x[n][3] - base[n][1]);
+                l[n][0] = fmaf(w0 + w2, apart[n][0] ? 0.f : ex2(ref[n][0] - lv), l[n][0]);
+                l[n][1] = fmaf(w1 + w3, apart[n][1] ? 0.f : ex2(ref[n][1] - lv), l[n][1]);
+                __half2 p0 = __floats2half2_rn(w0, w1), p1 = __floats2half2_rn(w2, w3);
+                const float2 fx = __half22float2(p0), fy = __half22float2(p1);
                 const __half2 rx = __floats2half2_rn(w0 - fx.x, w1 - fx.y), ry = __floats2half2_rn(w2 - fy.x, w3 - fy.y);
                 if (DUP) {  // columns 4-7: what the rounding of columns 0-3 left over
-                    x = t >= 2 ? rx : x;
-                    y = t >= 2 ? ry : y;
+                    p0 = t >= 2 ? rx : p0;
+                    p1 = t >= 2 ? ry : p1;
                 } else {    // ... of all columns: a second B operand
                     pr[n][0] = transpose8x8(half2_bits(rx));
                     pr[n][1] = transpose8x8(half2_bits(ry));
                 }
-                pb[n][0] = transpose8x8(half2_bits(x));
-                pb[n][1] = transpose8x8(half2_bits(y));
+                pb[n][0] = transpose8x8(half2_bits(p0));
+                pb[n][1] = transpose8x8(half2_bits(p1));
             }
             // ---- O^T += V^T P^T: row tile c has dim 16 c + 2 g in its row g and dim 16 c + 2 g + 1 in its row g + 8
             // Behind the sequence's end any byte may stand, an e4m3 NaN among them, and 0 x NaN is NaN.
@@ -795,18 +829,21 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_q8_kernel(const __gri
                 for (int e = 0; e < 2; ++e) {
                     const int head = n * 8 + 2 * t + e;
                     if (head >= heads || head >= HC) continue;
+                    // 2^ref in two factors: as one it may be too small for fp32 where the output is not.  (Where no value has had
+                    // a weight ref is no scale's, and the output 0: it has to be finite.)
+                    const float up = ex2(0.5f * fminf(ref[n][e], 126.f)), unit = (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f) * up;
                     if (whole) {
-                        const float f = (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f) / l[n][e];
+                        const float f = unit / l[n][e];
                         T *dst = (T *)p.o + ((int64_t)b * p.num_q_heads + hq0 + head) * D + 2 * g;
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) store2<T>(dst + 16 * i, o[n][i][e] * f, o[n][i][e + 2] * f);
+                        for (int i = 0; i < MT; ++i) store2<T>(dst + 16 * i, o[n][i][e] * f * up, o[n][i][e + 2] * f * up);
                     } else {
-                        const float f = l[n][e] == 0.f ? 0.f : (CODE == MKV_Q8_INT8 ? kCodeUnit : 1.f) / l[n][e];
+                        const float f = l[n][e] == 0.f ? 0.f : unit / l[n][e];
                         float *dst = row + head * D + 2 * g;
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
-                            *reinterpret_cast<float2 *>(dst + 16 * i) = make_float2(o[n][i][e] * f, o[n][i][e + 2] * f);
-                        if (g == 0) row[HC * D + head] = log2f(l[n][e]) + base[n][e];
+                            *reinterpret_cast<float2 *>(dst + 16 * i) = make_float2(o[n][i][e] * f * up, o[n][i][e + 2] * f * up);
+                        if (g == 0) row[HC * D + head] = l[n][e] == 0.f ? -INFINITY : log2f(l[n][e]) + (base[n][e] - ref[n][e]);
                     }
                 }
         }

@@ -84,12 +84,11 @@ def scales(c, name, exponents):
 
 # groups of 2, 8 and 16 on the tensor cores in both dims, and the plain kernel
 EXTREME = [(4, 2, 128), (4, 2, 64), (8, 1, 128), (16, 1, 128), (16, 1, 64), (4, 2, 80)]
-PLAIN = EXTREME[-1:]
 EXTREME_LENS = [1, 16, 17, 40, 100, 333, 64]
 
 
 @pytest.mark.parametrize("code", CODES)
-@pytest.mark.parametrize("hq,hkv,d", PLAIN)
+@pytest.mark.parametrize("hq,hkv,d", EXTREME)
 @pytest.mark.parametrize("exponents", [range(-126, -109), range(108, 119), range(-40, 11), range(-126, 119), [-126, 118]],
                          ids=["tiny", "huge", "spread", "all", "both ends"])
 def test_attention_takes_every_scale_of_v(mk, code, hq, hkv, d, exponents):  # noqa: F811
@@ -111,3 +110,73 @@ def test_attention_takes_every_scale_of_k(mk, code, hq, hkv, d, exponent):  # no
     q = (q * 2.0 ** (-exponent // 2) * 2.0 ** (-7 - exponent - (-exponent // 2))).to(torch.bfloat16)
     q[1], q[4, 1], q[5, -1] = 0, 0, 0
     check_32(c, c.attend(mk, q, c.state()), q.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hq,hkv,d", EXTREME)
+def test_attention_over_all_zero_blocks(mk, code, hq, hkv, d):  # noqa: F811
+    """Blocks of zeros have the scale 0: among others, a whole sequence of them, and with what a recycled page holds."""
+    c = Case(code, EXTREME_LENS + [50, 48], hq=hq, hkv=hkv, d=d, seed=d + hq + 2)
+    for g, s in zip(c.gpu, c.segs):
+        for name, codes in (("ks", "k"), ("vs", "v")):
+            zero = c.rs.rand(*s[name].shape) < 0.4
+            for i in (1, 7, 8):
+                for lb in range(-(-c.lens[i] // c.bs)):
+                    zero[c.table[c.ids[i], lb]] = name == "vs" or i == 8
+            s[name][zero] = 0
+            stale = c.rs.rand(*s[name].shape) < 0.3         # (not what store leaves, but 0 times it is 0 as well)
+            s[codes][zero & ~stale] = 0
+            g[name].copy_(c._dev(s[name])), g[codes].copy_(c._codes(s[codes]))
+    q, qn = c.rows(len(c.lens), hq, torch.bfloat16)
+    o = c.attend(mk, q, c.state())
+    check_32(c, o, qn)
+    assert (o[[1, 7, 8]] == 0).all()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hq,hkv,d", EXTREME)
+@pytest.mark.parametrize("nats", [5, 20, 31, 35, 42])
+def test_attention_where_the_heaviest_tokens_have_the_smallest_values(mk, code, hq, hkv, d, nats):  # noqa: F811
+    """A few blocks hold scores 2 * nats above all others', and values that are next to nothing or 0."""
+    c = Case(code, [333, 100, 64, 48, 200, 33], hq=hq, hkv=hkv, d=d, seed=d + hq + nats)
+    q = np.zeros((len(c.lens), hq, d))
+    q[:, :, 0] = 16
+    unit = nats / (127 * 16 * c.scale)
+    code_of = (lambda x: np.int8(x).view(np.uint8)) if code == "int8" else (lambda x: O.encode(np.float64(x), 1.0, "e4m3"))
+    for s in c.segs:
+        s["ks"][:] = np.float32(unit) if code == "int8" else np.float32(2.0 ** np.floor(np.log2(unit)))
+        s["k"][..., 0] = code_of(-127)
+    for i, n in enumerate(c.lens):
+        blocks = -(-n // c.bs)
+        for lb, exponent in zip(c.rs.permutation(blocks)[:3], [(-120, -100, -95), (-60,), (None, None, None), (None, -110), (-126, -120), (None,)][i]):
+            seg, r = O.page(c.segs, c.table, c.ids[i], lb)
+            seg["k"][r, c.layer, ..., 0] = c.rs.choice([code_of(127), code_of(120), code_of(104)], seg["k"][r, c.layer, ..., 0].shape)
+            seg["vs"][r, c.layer] = 0 if exponent is None else 2.0 ** exponent
+            if exponent is None:
+                seg["v"][r, c.layer] = 0
+    for g, s in zip(c.gpu, c.segs):
+        for name in ("k", "v"):
+            g[name].copy_(c._codes(s[name]))
+        for name in ("ks", "vs"):
+            g[name].copy_(c._dev(s[name]))
+    qt = torch.from_numpy(q).to(torch.bfloat16).cuda()
+    check_32(c, c.attend(mk, qt, c.state()), q)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hq,hkv,d", EXTREME)
+def test_attention_keeps_what_is_not_finite_among_zero_blocks(mk, code, hq, hkv, d):  # noqa: F811
+    """A key block that was not finite makes its row NaN although its values are 0: alone, as the first and as the last block."""
+    c = Case(code, [16, 40, 40, 40], hq=hq, hkv=hkv, d=d, seed=d + hq + 3)
+    s, g = c.segs[0], c.gpu[0]
+    for i, lb in ((0, 0), (1, 0), (2, 2)):
+        r = c.table[c.ids[i], lb]
+        s["ks"][r, c.layer], s["vs"][r, c.layer], s["v"][r, c.layer] = np.nan, 0, 0
+    s["vs"][c.table[c.ids[3], :2], c.layer] = 0
+    s["v"][c.table[c.ids[3], :2], c.layer] = 0
+    for name in ("ks", "vs"):
+        g[name].copy_(c._dev(s[name]))
+    g["v"].copy_(c._codes(s["v"]))
+    q, qn = c.rows(4, hq, torch.bfloat16)
+    o = c.attend(mk, q, c.state()).double().cpu().numpy().reshape(4, -1)
+    assert np.isnan(o[:3]).all() and not np.isnan(o[3]).any()
