@@ -10,6 +10,8 @@ consecutive ids, :473-504); the choice between the plain and the elastic copy ro
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 import numpy as np
@@ -17,6 +19,32 @@ import numpy as np
 from .. import swiftllm_c
 from .block_manager import BlockManager
 from .infer_state import LlamaInferState, seq_block_size_heuristic
+from .kernels.rotary_pos import rotary_inv_freq
+
+
+def make_rotary_tables(model_config, device):
+    """cos / sin tables, fp32 angles rounded to fp16 (worker/model.py:229-241).
+
+    ``rope_scaling`` is a number there (linear scaling, tables for as many positions more).  A mapping is taken too: linear
+    scaling by its factor is the same thing, the other types of ``rotary_inv_freq`` give its frequencies, times its factor
+    on sines and cosines, for all positions that the longer of ``max_position_embeddings`` and the scaled original stands for."""
+    mc = model_config
+    scaling = getattr(mc, "rope_scaling", 1) or 1
+    max_seq_len = getattr(mc, "max_position_embeddings", 4096)
+    if not isinstance(scaling, (int, float)):
+        inv_freq, factor = rotary_inv_freq(mc, device)
+        kind, scale = scaling.get("rope_type", scaling.get("type", "default")), float(scaling.get("factor", 1.0))
+        if kind not in ("default", "linear"):
+            original = scaling.get("original_max_position_embeddings") or max_seq_len
+            t = torch.arange(max(max_seq_len, math.ceil(original * scale)) + 128, device=device, dtype=torch.float64)
+            freqs = torch.outer(t, inv_freq)
+            return tuple((f(freqs) * factor).to(torch.float16) for f in (torch.cos, torch.sin))
+        scaling = scale if kind == "linear" else 1
+    base = getattr(mc, "rope_theta", 10000.0)
+    inv_freq = 1.0 / (base ** (torch.arange(0, mc.head_dim, 2, device=device, dtype=torch.float32) / mc.head_dim))
+    t = torch.arange(max_seq_len * scaling + 128, device=device, dtype=torch.float32) / scaling
+    freqs = torch.outer(t, inv_freq)
+    return torch.cos(freqs).to(torch.float16), torch.sin(freqs).to(torch.float16)
 
 
 class KVCacheModelState:
@@ -38,16 +66,7 @@ class KVCacheModelState:
 
     @torch.inference_mode()
     def _init_to_get_rotary(self):
-        """cos / sin tables, fp32 angles rounded to fp16 (worker/model.py:229-241)."""
-        mc = self.model_config
-        scaling = getattr(mc, "rope_scaling", 1) or 1
-        base = getattr(mc, "rope_theta", 10000.0)
-        max_seq_len = getattr(mc, "max_position_embeddings", 4096) * scaling
-        inv_freq = 1.0 / (base ** (torch.arange(0, mc.head_dim, 2, device="cuda", dtype=torch.float32) / mc.head_dim))
-        t = torch.arange(max_seq_len + 128, device="cuda", dtype=torch.float32) / scaling
-        freqs = torch.outer(t, inv_freq)
-        self._cos_cached = torch.cos(freqs).to(torch.float16)
-        self._sin_cached = torch.sin(freqs).to(torch.float16)
+        self._cos_cached, self._sin_cached = make_rotary_tables(self.model_config, "cuda")
 
     def _stage(self, n: int):
         """A pinned int32 buffer of at least n entries whose previous upload has finished (two take turns)."""
@@ -61,7 +80,7 @@ class KVCacheModelState:
 
     @torch.inference_mode()
     def prepare_step(self, input_ids_list, seq_ids_list, decoding_seq_lens_list, ignore_kvcache: bool = False,
-                     sync_free: bool = False) -> LlamaInferState:
+                     sync_free: bool = False, rotary_tables: bool = True) -> LlamaInferState:
         """The part of the reference's ``forward`` that turns its Python lists into the step's metadata and block
         allocation (worker/model.py:318-436): prefill sequences come first in ``input_ids_list``, decoding ones
         after them with one token each.  Returns the LlamaInferState the kernels of this package take.
@@ -69,7 +88,9 @@ class KVCacheModelState:
         Underneath, all integer metadata (sequence ids, lengths, prompt start offsets, token positions) is laid out
         in ONE pinned buffer on the host and uploaded with ONE asynchronous copy; the reference builds six small
         tensors from lists and derives the rest with cumsum / arange / cat kernels.  ``sync_free`` takes the
-        allocation path without a host round trip (errors then surface with the next ``num_free_blocks`` read)."""
+        allocation path without a host round trip (errors then surface with the next ``num_free_blocks`` read).
+        ``rotary_tables=False`` leaves ``position_cos`` and ``position_sin`` out (None), for steps that rotate by
+        ``positions`` (``rotary_embedding_positions``): no table is made or gathered from, or limits the positions."""
         mc = self.model_config
         n_dec = len(decoding_seq_lens_list)
         n_pre = len(input_ids_list) - n_dec
@@ -77,6 +98,12 @@ class KVCacheModelState:
         batch = n_pre + n_dec
         n_pre_tok = sum(prompt_lens)
         n_tok = n_pre_tok + n_dec
+        if rotary_tables:
+            if self._cos_cached is None:
+                self._init_to_get_rotary()
+            longest = max(max(prompt_lens, default=0), max(decoding_seq_lens_list, default=0))
+            if longest > self._cos_cached.shape[0]:
+                raise RuntimeError(f"a sequence of {longest} tokens is longer than the rotary tables ({self._cos_cached.shape[0]} positions)")
         # [ seq_ids | seq_lengths | prompt starts + end | token positions ]
         total = 2 * batch + (n_pre + 1) + n_tok
         host, done = self._stage(total)
@@ -105,8 +132,6 @@ class KVCacheModelState:
                 self.gpu_block_manager.allocate_blocks_for_seqs_nosync(seq_ids, seq_lengths)
             else:
                 self.gpu_block_manager.allocate_blocks_for_seqs(seq_ids, seq_lengths)
-        if self._cos_cached is None:
-            self._init_to_get_rotary()
         seq_block_size, num_seq_blocks = seq_block_size_heuristic(mc.num_kv_heads, decoding_seq_lens_list)
         state = LlamaInferState(
             batch_size=batch, num_tokens=n_tok, seq_ids=seq_ids, softmax_scale=mc.head_dim ** -0.5,
@@ -117,7 +142,8 @@ class KVCacheModelState:
             num_seq_blocks=num_seq_blocks,
             num_blocks_org=self.gpu_block_manager.num_blocks_org if self.gpu_block_manager else None,
             kv_cache_new_block_size=self.kv_cache_new_block_size, org_layer_param_size=self.org_layer_param_size,
-            position_cos=self._cos_cached[positions], position_sin=self._sin_cached[positions],
+            position_cos=self._cos_cached[positions] if rotary_tables else None,
+            position_sin=self._sin_cached[positions] if rotary_tables else None,
             ignore_kvcache=ignore_kvcache)
         state.positions = positions     # int32 [num_tokens], for rotary_embedding_positions; not a field of the reference's class
         return state

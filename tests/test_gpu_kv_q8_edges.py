@@ -1,4 +1,6 @@
 """GPU: calls of the 8-bit pool's operators at the far ends of what they accept."""
+import types
+
 import numpy as np
 import pytest
 import torch
@@ -50,3 +52,42 @@ def test_a_length_hint_far_above_the_lengths(mk, bs):  # noqa: F811
     want = [np.concatenate([a, b[3:]]) for a, b in zip(*(O.cached(c.segs, "int8", c.table, i, n, c.layer, bs)[:2] for i, n in zip(c.ids, (7, 20))))]
     for got, w in zip((k, v), want):
         assert (np.abs(got[:24].double().cpu().numpy() - w) <= (2.0 ** -11 + 2.0 ** -23) * np.abs(w) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("scaling", [None, 2.0, {"type": "linear", "factor": 2.0}, {"rope_type": "ntk", "factor": 2.0},
+                                     {"rope_type": "llama3", "factor": 8.0, "original_max_position_embeddings": 64},
+                                     {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 64}],
+                         ids=["none", "number", "linear", "ntk", "llama3", "yarn"])
+def test_a_step_with_scaled_frequencies(mk, scaling):  # noqa: F811
+    """One model configuration for rotary_inv_freq and the model state's steps: positions and tables say the same."""
+    mc = types.SimpleNamespace(num_layers=1, num_q_heads=4, num_kv_heads=2, head_dim=64, max_position_embeddings=256, rope_scaling=scaling)
+    ec = types.SimpleNamespace(block_size=16, max_blocks_per_seq=16, max_seqs_in_block_table=6, num_cpu_blocks=2)
+    state = mk.KVCacheModelState(mc, ec)
+    state.gpu_block_manager = mk.BlockManager("GPU", 40, 6, 16, 16)
+    inv, att = mk.rotary_inv_freq(mc)
+    st = state.prepare_step([[0] * 100, [0]], [2, 4], [200])
+    assert st.positions.tolist() == list(range(100)) + [199]
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k = (torch.randn((101, h, 64), device="cuda", generator=gen, dtype=torch.float16) for h in (4, 2))
+    q2, k2 = q.clone(), k.clone()
+    mk.rotary_embedding_inplace(q2, k2, st)
+    size = (q.float().abs() + q.float().abs().roll(32, -1), k.float().abs() + k.float().abs().roll(32, -1))
+    mk.rotary_embedding_positions(q, k, st.positions, inv, attention_scale=att)
+    for a, b, s in zip((q, k), (q2, k2), size):
+        # tables: fp16 cosines of fp32 angles (2^-11, and 199 * 2^-24 twice); fp16 arithmetic on one side, one rounding on the other
+        assert ((a.float() - b.float()).abs() <= att * s * 4 * 2.0 ** -11).all()
+    st = state.prepare_step([[0], [0]], [2, 4], [101, 201], rotary_tables=False)
+    assert st.position_cos is None and st.position_sin is None and st.positions.tolist() == [100, 200]
+
+
+def test_a_step_beyond_the_rotary_tables_is_refused_on_the_host(mk):  # noqa: F811
+    mc = types.SimpleNamespace(num_layers=1, num_q_heads=4, num_kv_heads=2, head_dim=64, max_position_embeddings=16, rope_scaling=None)
+    ec = types.SimpleNamespace(block_size=16, max_blocks_per_seq=16, max_seqs_in_block_table=6, num_cpu_blocks=2)
+    state = mk.KVCacheModelState(mc, ec)
+    state.gpu_block_manager = mk.BlockManager("GPU", 40, 6, 16, 16)
+    free = state.gpu_block_manager.num_free_blocks
+    with pytest.raises(RuntimeError, match="rotary tables"):
+        state.prepare_step([[0]], [1], [145])
+    assert state.gpu_block_manager.num_free_blocks == free
+    assert state.prepare_step([[0]], [1], [144]).position_cos.shape == (1, 32)
+    assert state.prepare_step([[0]], [1], [200], rotary_tables=False).positions.tolist() == [199]

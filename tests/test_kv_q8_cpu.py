@@ -218,3 +218,27 @@ def test_yarn_variants_are_refused(mk):
         with pytest.raises(ValueError):
             mk.rotary_inv_freq(cfg(rope_scaling={**sc, **more}), device="cpu")
     assert mk.rotary_inv_freq(cfg(rope_scaling={**sc, "truncate": True, "mscale": None}), device="cpu")[1] > 1
+
+
+# ------------------------------------------------------------------------------------------- the model state's tables
+def test_rotary_tables_take_the_scaling_mappings(mk):
+    from morphserve_b200.worker.kv_model import make_rotary_tables
+    plain = make_rotary_tables(cfg(), "cpu")
+    assert all(torch.equal(a, b) for a, b in zip(plain, make_rotary_tables(cfg(rope_scaling={"rope_type": "default"}), "cpu")))
+    assert plain[0].shape == (4096 + 128, 64) and plain[0].dtype == torch.float16
+    number = make_rotary_tables(cfg(rope_scaling=4.0), "cpu")
+    assert number[0].shape[0] == 4 * 4096 + 128
+    assert all(torch.equal(a, b) for a, b in zip(number, make_rotary_tables(cfg(rope_scaling={"type": "linear", "factor": 4.0}), "cpu")))
+    for sc, rows in (({"rope_type": "ntk", "factor": 2.5}, 10240),
+                     ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+                       "original_max_position_embeddings": 512}, 4096),
+                     ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 2048}, 8192)):
+        inv, att = mk.rotary_inv_freq(cfg(rope_scaling=sc), device="cpu")
+        angles = np.outer(np.arange(rows + 128, dtype=np.float64), inv.numpy())
+        got = make_rotary_tables(cfg(rope_scaling=sc), "cpu")
+        for f, t in zip((np.cos, np.sin), got):
+            assert t.shape == angles.shape and t.dtype == torch.float16 and t.is_contiguous()
+            # one rounding to fp16; angles up to 10^4 in 64 bits
+            assert (np.abs(t.double().numpy() - f(angles) * att) <= 2.0 ** -11 * np.abs(f(angles) * att) + 2.0 ** -25 + 1e-11).all()
+    with pytest.raises(ValueError):
+        make_rotary_tables(cfg(rope_scaling={"rope_type": "other", "factor": 2.0}), "cpu")
