@@ -352,7 +352,7 @@ int mkv_store_kv_prefill(int device, void *stream, const void *k, const void *v,
  * k_stride / v_stride elements apart.  table_stride = columns of the block table, num_rows = its rows.
  * Prefill: every block a prompt touches gets its scale from the prompt's tokens alone; slots behind the prompt's end keep
  * their bytes.  Prompt i takes rows [start_locs[i], start_locs[i] + seq_lens[i]) of k and v; rows at or behind
- * num_tokens are not read.  max_seq_len only sizes the launch.
+ * num_tokens are not read.  max_seq_len only sizes the launch; 0 says that there is nothing to store.
  * Decode: token len-1 of every sequence is appended.  In the first slot of a block its scale starts from the new token;
  * later the larger of the block's and the token's scale holds, and if that is the token's, the codes of the slots
  * before it are rounded again to the new scale (int8: q * fl32(old * fl32(1 / new)); e4m3: q * old / new).
@@ -371,7 +371,7 @@ int mkv_store_kv_q8_decode(int device, void *stream, const void *k, const void *
  * Cached tokens back into contiguous rows: token t in [begins[i], ends[i]) of sequence seq_ids[i] becomes row
  * start_locs[i] + t - begins[i] of k and v ([num_out_rows, num_kv_heads, head_dim] of `dtype`, rounded once from
  * q * scale).  Rows at or behind num_out_rows, and tokens whose page is not there (as above), are not written.
- * max_len (the longest range) only sizes the launch.
+ * max_len (the longest range) only sizes the launch; 0 says that there is nothing to load.
  */
 int mkv_load_kv_q8(int device, void *stream, void *k, void *v, int64_t k_stride, int64_t v_stride, int dtype,
                    int64_t num_out_rows, const mkv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,

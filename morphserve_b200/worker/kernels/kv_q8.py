@@ -155,7 +155,8 @@ def store_kvcache_q8(
         status = lib.mkv_store_kv_q8_prefill(
             dev, stream, k.data_ptr(), v.data_ptr(), ks, vs, dtype, n_tok, pool, table, cols, rows, seq_ids,
             _ints(infer_state.prefill_seq_start_locs, dev, n_pre, "prefill_seq_start_locs"),
-            _ints(infer_state.prefill_seq_lens, dev, n_pre, "prefill_seq_lens"), n_pre, int(infer_state.max_prefill_len), cur_layer)
+            _ints(infer_state.prefill_seq_lens, dev, n_pre, "prefill_seq_lens"), n_pre,
+            int(infer_state.max_prefill_len) or 1, cur_layer)     # (sizes the launch; 0 would be none)
         check(status, "mkv_store_kv_q8_prefill")
     if n_dec > 0:
         skip = n_tok * k.element_size()
@@ -201,7 +202,7 @@ def load_kvcache_q8(
     check(lib.mkv_load_kv_q8(
         dev, raw_stream(dev), k.data_ptr(), v.data_ptr(), ks, vs, dtype, k.shape[0], pool, table, cols, rows,
         _ints(seq_ids, dev, n, "seq_ids"), _ints(begins, dev, n, "begins"), _ints(ends, dev, n, "ends"),
-        _ints(start_locs, dev, n, "start_locs"), n, int(max_len), cur_layer), "mkv_load_kv_q8")
+        _ints(start_locs, dev, n, "start_locs"), n, int(max_len) or 1, cur_layer), "mkv_load_kv_q8")
 
 
 def paged_attention_q8(

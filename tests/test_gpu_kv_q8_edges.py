@@ -91,3 +91,20 @@ def test_a_step_beyond_the_rotary_tables_is_refused_on_the_host(mk):  # noqa: F8
     assert state.gpu_block_manager.num_free_blocks == free
     assert state.prepare_step([[0]], [1], [144]).position_cos.shape == (1, 32)
     assert state.prepare_step([[0]], [1], [200], rotary_tables=False).positions.tolist() == [199]
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_a_length_hint_of_zero(mk, code):  # noqa: F811
+    """... stores and loads what the lengths say all the same."""
+    c = Case(code, [7, 40], hkv=2, d=32, seed=42)
+    k, kn = c.rows(47, 2, torch.float16)
+    v, vn = c.rows(47, 2, torch.float16)
+    st = c.state(prefill=[7, 40], decode=[])
+    st.max_prefill_len = 0
+    mk.store_kvcache_q8(k, v, *c.pool(), c.table_t, c.mc, c.ec, st, c.layer)
+    O.store_prefill(c.segs, code, kn, vn, c.table, c.ids, [0, 7], [7, 40], c.layer, c.bs)
+    c.same()
+    k.zero_(), v.zero_()
+    mk.load_kvcache_q8(k, v, *c.pool(), c.table_t, c.mc, c.ec, i32(c.ids[1:]), i32([0]), i32([40]), i32([7]), 0, c.layer)
+    for got, want in zip((k, v), O.cached(c.segs, code, c.table, c.ids[1], 40, c.layer, c.bs)):
+        assert (np.abs(got[7:].double().cpu().numpy() - want) <= (2.0 ** -11 + 2.0 ** -23) * np.abs(want) + 2.0 ** -25).all()
