@@ -399,7 +399,7 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
 
 /*
  * Rotary embedding by position: pair j of every head of token t turns by the angle positions[t] * inv_freq[j]
- * (64 bits, reduced to a fraction of a turn before it is rounded) and is scaled by attention_scale; computed in fp32,
+ * (exact up to positions of 2^53 and frequencies of 1, reduced to a fraction of a turn, then rounded) and is scaled by attention_scale; computed in fp32,
  * rounded once.  num_pairs = elements of inv_freq = rotary dimensions / 2; elements behind 2 * num_pairs pass through.
  * Pairs are (j, j + num_pairs), or with interleaved != 0 (2j, 2j + 1).  strides (host, 8): elements between tokens and
  * between heads of q, k, q_out, k_out.  q_out / k_out: q / k themselves (in place) or memory that overlaps neither.

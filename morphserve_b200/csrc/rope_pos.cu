@@ -1,7 +1,8 @@
 // Rotary embedding by position: no tables.  Pair j of token t turns by positions[t] * inv_freq[j].
 //
 // The angle is formed in 64 bits and reduced to a fraction of a turn there: a position of 10^5..10^6 leaves a 32-bit
-// product without correct digits behind the point, while here the reduced angle is good to 2^-24 of half a turn.  One
+// product without correct digits behind the point, while here the reduced angle is good to 2^-24 of half a turn for positions of
+// up to 2^53 and frequencies of up to 1 (in 64 bits to 2^-53 of a turn: the product keeps what its rounding leaves over).  One
 // thread block computes the sines and cosines of its tokens once, in shared memory, for all heads of q and k; its first
 // row loads are in flight meanwhile.  HBM bound: every element is read and written once.
 #include <algorithm>
@@ -138,11 +139,11 @@ __global__ void __launch_bounds__(kRopeThreads, sizeof(T) * V <= 16 ? kRopeBlock
         const int tk = i / p.num_pairs;
         const double pos = p.pos64 ? (double)((const int64_t *)p.positions)[tok0 + tk]
                                    : (double)((const int32_t *)p.positions)[tok0 + tk];
-        // a radians are a / 2 pi turns; 1 / 2 pi in two parts, so that the fraction keeps its digits however many whole
-        // turns go away
+        // a + e radians, e what the product's rounding leaves over, are (a + e) / 2 pi turns; 1 / 2 pi in two parts, so that the
+        // fraction keeps its digits however many whole turns go away
         const int pair = i - tk * p.num_pairs;
-        const double a = pos * p.inv_freq[pair];
-        const double x = fma(a, 0.15915494309189535, -rint(a * 0.15915494309189535)) + a * -9.839338337591243e-18;
+        const double f = p.inv_freq[pair], a = pos * f, e = fma(pos, f, -a);
+        const double x = fma(a, 0.15915494309189535, -rint(a * 0.15915494309189535)) + fma(a, -9.839338337591243e-18, e * 0.15915494309189535);
         float sn, cs;
         sincospif((float)(2.0 * x), &sn, &cs);
         turns[tk * p.num_pairs + (pair % V) * p.pair_tasks + pair / V] = make_float2(cs * p.scale, sn * p.scale);

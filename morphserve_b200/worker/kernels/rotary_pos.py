@@ -111,8 +111,8 @@ def rotary_embedding_positions(
     """Rotate pair j of every head of token t by ``positions[t] * inv_freq[j]`` and scale it by ``attention_scale``;
     elements behind the rotated part pass through unchanged.  In place, or into ``q_out`` / ``k_out`` (memory that does
     not overlap q and k).  fp16, bf16 or fp32, computed in fp32 and rounded once.  Elements are contiguous; tokens and
-    heads may lie any distance apart, so q and k may be views of one fused projection.  Any position that a 64-bit float
-    holds keeps its angle to about 2^-24 of half a turn."""
+    heads may lie any distance apart, so q and k may be views of one fused projection.  Positions of up
+    to 2^53 (what a 64-bit float counts) and frequencies of up to 1 give the angle to about 2^-24 of half a turn."""
     dev = q.get_device()
     if dev < 0:
         require_cuda(q, "q")

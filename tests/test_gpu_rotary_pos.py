@@ -1,4 +1,6 @@
 """GPU parity of the rotary embedding by position against the 64-bit oracle."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
@@ -118,3 +120,22 @@ def test_in_a_graph(mk):
         g.replay()
         torch.cuda.synchronize()
         check(qo, qn, np.arange(first, first + 12), inv, False, 1.0)
+
+
+def test_positions_up_to_what_64_bits_count(mk):
+    """Frequencies with all their digits: the angle is the exact product's, however many turns it has."""
+    rs = np.random.RandomState(3)
+    pos = np.concatenate([rs.randint(2 ** b, 2 ** (b + 1), 6) for b in (20, 31, 36, 40, 44, 48, 52)] + [[2 ** 53, -2 ** 53, 2 ** 53 - 1]])
+    inv = np.sort(rs.uniform(0.001, 1, 32))[::-1].copy()
+    n = len(pos)
+    q, k = (torch.from_numpy(rs.randn(n, h, 64)).float().cuda() for h in (2, 1))
+    qn = q.double().cpu().numpy()
+    mk.rotary_embedding_positions(q, k, torch.from_numpy(pos).cuda(), torch.from_numpy(inv).cuda())
+    # the product as a fraction, its remainder of a turn with 70 digits of pi
+    turn = 2 * Fraction("3.1415926535897932384626433832795028841971693993751058209749445923078164")
+    angle = np.array([[float(Fraction(int(p)) * Fraction(float(f)) % turn) for f in inv] for p in pos])
+    c, s = np.cos(angle)[:, None], np.sin(angle)[:, None]
+    a, b = qn[..., :32], qn[..., 32:]
+    want = np.concatenate([a * c - b * s, a * s + b * c], -1)
+    size = np.concatenate([np.abs(a) + np.abs(b)] * 2, -1)
+    assert (np.abs(q.double().cpu().numpy() - want) <= (2.0 ** -20 + 2.0 ** -24) * size).all()     # (as in check())
