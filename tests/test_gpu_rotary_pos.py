@@ -139,3 +139,18 @@ def test_positions_up_to_what_64_bits_count(mk):
     want = np.concatenate([a * c - b * s, a * s + b * c], -1)
     size = np.concatenate([np.abs(a) + np.abs(b)] * 2, -1)
     assert (np.abs(q.double().cpu().numpy() - want) <= (2.0 ** -20 + 2.0 ** -24) * size).all()     # (as in check())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("n,hq,hkv,d,rd", [(7109, 2, 1, 128, 128), (10657, 3, 2, 32, 16), (14211, 1, 1, 80, 64), (30000, 1, 1, 8, 2)])
+def test_several_tokens_a_thread_block(mk, dtype, interleaved, n, hq, hkv, d, rd):
+    """Enough tokens for blocks of two and more of them, the last one cut."""
+    rs = np.random.RandomState(n)
+    qkv = torch.from_numpy(rs.randn(n, hq + hkv, d)).to(dtype).cuda()
+    q, k = qkv[:, :hq], qkv[:, hq:]
+    qn, kn = q.double().cpu().numpy(), k.double().cpu().numpy()
+    pos, inv = rs.randint(0, 100000, n), inv_freq(rd)
+    mk.rotary_embedding_positions(q, k, torch.from_numpy(pos).cuda(), torch.from_numpy(inv).cuda(), interleaved=interleaved)
+    check(q, qn, pos, inv, interleaved, 1.0)
+    check(k, kn, pos, inv, interleaved, 1.0)
