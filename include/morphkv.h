@@ -369,8 +369,8 @@ int mkv_store_kv_q8_decode(int device, void *stream, const void *k, const void *
 
 /*
  * Cached tokens back into contiguous rows: token t in [begins[i], ends[i]) of sequence seq_ids[i] becomes row
- * start_locs[i] + t - begins[i] of k and v ([num_out_rows, num_kv_heads, head_dim] of `dtype`, rounded once from
- * q * scale).  Rows at or behind num_out_rows, and tokens whose page is not there (as above), are not written.
+ * start_locs[i] + t - begins[i] of k and v ([num_out_rows, num_kv_heads, head_dim] of `dtype`, rounded from the
+ * fp32 product q * scale).  Rows at or behind num_out_rows, and tokens whose page is not there (as above), are not written.
  * max_len (the longest range) only sizes the launch; 0 says that there is nothing to load.
  */
 int mkv_load_kv_q8(int device, void *stream, void *k, void *v, int64_t k_stride, int64_t v_stride, int dtype,
@@ -379,8 +379,8 @@ int mkv_load_kv_q8(int device, void *stream, void *k, void *v, int64_t k_stride,
                    const int32_t *start_locs, int num_seqs, int max_len, int cur_layer);
 
 /*
- * Decode attention over the 8-bit pool: one query token for each sequence, o = softmax(scale * q (s K)^T) (s V) in
- * fp32, rounded once to `dtype`.  q: [batch, num_q_heads, head_dim], sequences q_stride elements apart; o contiguous.
+ * Decode attention over the 8-bit pool: one query token for each sequence, o = softmax(scale * q (s K)^T) (s V) with
+ * sums in fp32 (weights on the fast path as an fp16 number and its remainder, 22 bits together), rounded once to `dtype`.  q: [batch, num_q_heads, head_dim], sequences q_stride elements apart; o contiguous.
  * The call plans, attends and merges in ONE launch.  `workspace` (device, 256-byte aligned, at least
  * mkv_attn_q8_workspace_bytes(...) bytes, whose first mkv_attn_q8_zero_bytes(...) bytes are zero before its first use and are
  * left zero by every call, the error word excepted) must not be shared by calls that may overlap on the GPU.

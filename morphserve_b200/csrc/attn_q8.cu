@@ -3,11 +3,11 @@
 // HBM bound: every code is read once for the query heads that share its kv head; what a token costs beyond its bytes is
 // the conversion of its codes to fp16, which is why the tensor-core tile is laid out for as few instructions as it is.
 //
-// Measured (B200, copy peak 6.55 TB/s): 256 sequences of up to 1536, 32 / 8 heads, int8: 402 MB in 82-88 us with the power cap
-// active all along; 64 sequences of up to 768, 32 heads, e4m3: 217 MB in 49.6 us; 8 sequences of 8 k to 32 k, 64 / 8 heads, e4m3:
-// 324 MB in 68 us (0.7 of the peak over all).  While it streams the kernel runs at the peak; the rest is the start (four
-// dependent reads before the first tile: 5 us), warps that end 8 to 10 % after the median (SMs differ so much in speed), and the
-// fold and merge of cut sequences (6 us).  8 sequences of up to 2048: 16.2 us, all of it such latencies.
+// Measured (B200, copy peak 6.55 TB/s; several GPUs): 256 sequences of up to 1536, 32 / 8 heads, int8: 402 MB in 83-88 us; 64
+// sequences of up to 768, 32 heads, e4m3: 217 MB in 50-51 us; 8 sequences of 8 k to 32 k, 64 / 8 heads, e4m3: 324 MB in 69-74 us
+// (0.7 of the peak over all).  While it streams the kernel runs at the peak; the rest is the start (four dependent reads before
+// the first tile: 5 us), warps that end 8 to 10 % after the median (SMs differ so much in speed, and equal shares do not even it
+// out), and the fold and merge of cut sequences (6 us).  8 sequences of up to 2048: 16.4 us, all of it such latencies.
 //
 // One launch.  The launch's tiles (32 tokens of one kv head: 32 x D codes of K and of V) stand in one order - sequence by
 // sequence, kv head by kv head, tile by tile, with a few phantom tiles in front of every (sequence, head) for what
@@ -1031,9 +1031,10 @@ constexpr size_t kErrorBytes = 256;     // error word, then the arrival counters
 static size_t zero_bytes(int sms) { return kErrorBytes + (((size_t)sms * kBlocksPerSm * sizeof(int) + 255) & ~(size_t)255); }
 // Query heads of a unit: 4, 8 or 16.  The weights enter the second product as an fp16 number and what that leaves over, also
 // fp16 (2^-22 of the weight together).  With 4 heads the remainders are columns 4-7 of the tile and cost nothing; with 8 and 16
-// they are a second B operand, twice the products of V: long contexts in groups of 8, e4m3 68.7 -> 73 us, int8 72 -> 80; 256
-// sequences in groups of 8 48.7 -> 53.5, of 16 65 -> 71.  Without them an output is off by 1.4e-4 of the weighted values' size,
-// which shows beside fp16's own rounding and is far above it where values cancel.
+// they are a second B operand, twice the products of V: without and with them (and what every scale of V takes), long contexts in
+// groups of 8 take 68-71 and 69-74 us (e4m3), 66 and 76 us (int8), 256 sequences in groups of 8 48 and 54 us, of 16 65 and 72 us.
+// Without them an output is off by 1.4e-4 of the weighted values' size, which shows beside fp16's own rounding and is far above
+// it where values cancel.
 static int unit_heads(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 
 static bool fast_shape(const PoolViewQ8 &pv) {
@@ -1159,7 +1160,7 @@ int mkv_paged_attention_q8(int device, void *stream, const void *q, int64_t q_st
         while ((kHalf << p.half_shift) < pv.block_size) ++p.half_shift;
         p.max_len = (int)std::min<int64_t>(table_stride * pv.block_size, 0x7fffffff);
         p.scale_log2 = scale_log2;
-        const int most = sms * kBlocksPerSm;    // (fast_positions keeps (most + 1) * step below 2^31)
+        const int most = sms * kBlocksPerSm;
         const int64_t positions = (int64_t)batch * (ceil_div64(max_seq_len, kTile) + kUnitCost) * pv.num_kv_heads * p.groups;
         const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, positions / (heads == 16 ? kWarpsWide : kWarps)));
         p.error_flags = (int *)workspace;

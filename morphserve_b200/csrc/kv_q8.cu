@@ -154,7 +154,8 @@ __device__ __forceinline__ bool named_again(const StoreQ8Args &a, int i, int row
 // grid = (pages of the longest prompt, prompts, heads / 8).  A warp takes one head of a page, K and then V: the rows go into registers with
 // every load in flight at once (NV pieces a thread; 4 KiB a warp at 16 x 128 fp16), the peak is a butterfly, the codes leave
 // as one contiguous tile.  NV = 0: pages that do not fit are read twice.
-// HBM bound: 64 prompts of up to 1536 tokens, 8 heads of 128 fp16, 54 us = 5.8 TB/s read and written (copy peak 6.55).
+// HBM bound: 64 prompts of up to 1536 tokens, 8 heads of 128 fp16, 54 us = 5.8 TB/s read and written (copy peak 6.55).  Half
+// occupancy (64 registers a thread): the variants with four pieces of 16-bit rows spill 12 to 16 bytes.
 template <typename T, int CODE, int V, int NV>
 __device__ __forceinline__ float store_tile(const StoreQ8Args &a, const T *src, int64_t stride, uint8_t *dst, int total, int vecs, int lane) {
     uint32_t peak = 0;
@@ -295,8 +296,8 @@ struct LoadQ8Args {
 
 // grid = (pages of the longest range, ranges, parts of a page).  A page is (head, K or V) tiles of `chunks` x 32 pieces (V codes
 // each); a warp takes kLoadFlight such chunks at a time, all of their loads before the first store.
-// Bound by writing: 16-bit rows are twice their codes, and the memory takes writes at 3.4-3.9 TB/s (a plain fill; reads and
-// writes in equal parts go at 6.5).  32 prefixes, 65 MB written: 22.4-24 us, a fill of those bytes alone 19.4 us.  A third of the
+// Bound by writing: 16-bit rows are twice their codes, and the memory takes writes at 3.5-3.9 TB/s (a plain fill of 33-200 MB;
+// reads and writes in equal parts go at 6.5).  32 prefixes, 65 MB written: 22.4 us, a fill of those bytes alone 17.6 us.  A third of the
 // instructions (the piece's place kept over the heads) changed nothing.
 template <typename T, int CODE, int V>
 __global__ void __launch_bounds__(kLoadThreads, 4) load_q8_kernel(const __grid_constant__ LoadQ8Args a) {

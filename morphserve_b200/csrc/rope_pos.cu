@@ -108,11 +108,12 @@ struct RopeTask {
 // block holds side by side.  Its first loads wait for nothing; the angles are formed while they are on their way.  One task
 // in flight a thread and every thread slot of the SM filled: 64 KiB in flight, which measured better than two or four tasks
 // in fewer threads (49600 tokens of 32 + 8 heads of 128 fp16: 164 us against 180 and 206 us; 154 us = 6.6 TB/s once the
-// arithmetic went by words).
+// arithmetic went by words).  Full occupancy leaves 32 registers a thread: the widest variants spill about 50 bytes of what
+// the loop keeps, which at the copy peak costs nothing.
 constexpr int kRopeThreads = 256, kRopeBlocks = 8;
 
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads, sizeof(T) * V <= 16 ? kRopeBlocks : 4) rope_pos_kernel(const __grid_constant__ RopePosArgs p) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_pos_kernel(const __grid_constant__ RopePosArgs p) {
     // (cos, sin) * scale of [token of the block][pair's place in its task][task]: the threads of a row read neighbours
     extern __shared__ float2 turns[];
     const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;

@@ -189,7 +189,8 @@ def load_kvcache_q8(
 ):
     """Cached tokens back as rows: token t of ``seq_ids[i]``, ``begins[i] <= t < ends[i]``, becomes row
     ``start_locs[i] + t - begins[i]`` of ``k`` and ``v`` - a cached prefix for a prefill attention that wants contiguous
-    rows, or a sequence on its way into another pool.  Rows that no range reaches, and rows of tokens whose page is not
+    rows, or a sequence on its way into another pool.  Values are the fp32 product of code and scale, rounded to the
+    rows' type.  Rows that no range reaches, and rows of tokens whose page is not
     in the table or the pool, are left as they were."""
     pool, shape, dev = _pool(k_cache, v_cache, k_scale, v_scale, k_cache_new, v_cache_new, k_scale_new, v_scale_new,
                              model_config, engine_config, k_cache.shape[0], k_cache_new[0].shape[0] if len(k_cache_new) else 0)
@@ -223,7 +224,7 @@ def paged_attention_q8(
     o: torch.Tensor,            # [num_decoding_seqs, num_q_heads(*)head_dim], written
 ):
     """Decode attention over the 8-bit pool, like ``paged_attention``: softmax(scale * q K^T) V of every decoding
-    sequence's one query token over its ``decoding_seq_lens`` cached tokens, in fp32, rounded once.
+    sequence's one query token over its ``decoding_seq_lens`` cached tokens, with scores and sums in fp32, rounded once.
 
     Rows of sequences of length 0 are left as they were.  A page that is not in the table or the pool takes no part
     (and is reported by ``read_attn_error_flags``); a row that is left without any token is NaN.
